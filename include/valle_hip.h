@@ -500,6 +500,70 @@ size_t valle_noalloc_scratch_bytes(void);
 int valle_ar_decode_noalloc(valle_model* m, const valle_ar_state* st, const valle_sample_params* sp,
                             int n_steps, float* logits_out, int ld_logits, void* stream);
 
+/* ------------------------------------------------------- paged KV cache and drafted tokens ---- */
+/* NO COUNTERPART IN THE REFERENCE (it recomputes the whole sequence per step, models/base.py:521 use_cache=False): the serving form
+ * of valle_rope_kv / valle_attn_decode, whose caches hold one contiguous slot per utterance.  Per layer
+ * kcache / vcache [n_pages][Hkv][page_size][64], page_size 16, 32, 64, 128 or 256; slot = page * page_size + offset;
+ * n_pages * page_size and max_blocks * page_size < 2^31 (offsets in elements are 64-bit).  Page numbers outside the pool are
+ * never followed: their rows are not written and count as absent. */
+
+/* Takes request b from len_old[b] to len_new[b] cached rows: pages beyond ceil(len_new / page_size) return to the free stack
+ * free_list[0 .. free_count), missing ones are popped in request order.  With F free pages after all returns, page x of the running
+ * numbering (of the returned ones, of the taken ones) is free_list[F - 1 - x].  Out:
+ *   block_table [B][max_blocks]  the new pages (entries at and behind n_blocks_out[b] are left), free_list
+ *   n_blocks_out [B], free_count_out [1]   may be n_blocks_in / free_count_in
+ *   status [B]                   0 served, 1 the stack ran dry in front of it (it keeps its pages), 2 lengths or n_blocks out of range (or more
+ *                                than 64 new rows with parents), 3 its rows end behind max_rows (2 and 3 change nothing of it)
+ *   cu_rows [B + 1]              prefix sums of max(0, len_new - len_old) (0 rows at status 2)
+ *   slots, positions [max_rows]  of row cu_rows[b] + i: slot and number of cached row len_old[b] + i; slot -1 for requests not
+ *                                served; -1 and position 0 behind the last row
+ * With parents [max_rows] (tree_mask [max_rows] then too): row i of a request is a node whose parent is its row parents[.], an
+ * earlier one (anything else: the context); its position is len_old + depth and tree_mask holds bit j for itself and every
+ * ancestor j.  B <= 4096.  One launch up to 4,096 rows, two beyond. */
+int valle_page_plan(const int32_t* len_old, const int32_t* len_new, int B, int page_size, int32_t* block_table, int max_blocks,
+                    const int32_t* n_blocks_in, int32_t* n_blocks_out, int32_t* free_list, int n_pages,
+                    const int32_t* free_count_in, int32_t* free_count_out, int32_t* status, int32_t* cu_rows,
+                    int32_t* slots, int32_t* positions, int max_rows, const int32_t* parents, int64_t* tree_mask, void* stream);
+
+/* valle_rope_kv for pages: q [M][H][64], k, v [M][Hkv][64] (row strides in elements, rows 16-byte aligned), q and k rotated by
+ * rope[positions[m]] ([rope_rows][32][2] fp32; a position outside takes the nearest row), q to q_out (q_out == q is allowed; both
+ * NULL: no q), k and v to slot slots[m] of the caches (a slot outside the pool: not written).  fp32 arithmetic, one rounding (in
+ * bf16 valle_rope_kv rounds cos and sin first: not bit-equal).  Slots must differ from one another. */
+int valle_rope_kv_paged(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride,
+                        void* q_out, int64_t q_out_row_stride, const int32_t* positions, const float* rope, int rope_rows,
+                        const int32_t* slots, int M, int H, int Hkv, int Dh, void* kcache, void* vcache, int n_pages, int page_size,
+                        int dtype, void* stream);
+
+/* Attention of drafted tokens over the pages: request b asks with rows cu_rows[b] .. cu_rows[b + 1] of q ([rows][H][64], up to
+ * max_nodes <= 64 of them; rows behind that are left), cached at positions ctx_len[b] + i of its pages.  A row sees the ctx_len[b]
+ * context rows and the nodes whose bit is set in its tree_mask (NULL: rows 0 .. itself); H % Hkv == 0, head h reads kv head
+ * h / (H / Hkv).  A row that sees nothing gives zeros; requests with ctx_len < 0 and rows of no request are left as they were.
+ * Rows of a page behind the sequence, and nodes a row does not see, may hold anything (infinities, NaN).  max_ctx: host-side
+ * estimate of the longest context; it only chooses how the keys are split.  workspace: valle_attn_tree_workspace_bytes with the
+ * same numbers (0: none needed), 16-byte aligned, not shared by calls that may overlap. */
+size_t valle_attn_tree_workspace_bytes(int rows, int B, int max_nodes, int max_ctx, int H, int Hkv, int dtype);
+int valle_attn_tree(const void* q, int64_t q_row_stride, const void* kcache, const void* vcache, int n_pages, int page_size,
+                    const int32_t* block_table, int max_blocks, const int32_t* ctx_len, const int32_t* cu_rows,
+                    const int64_t* tree_mask, void* out, int64_t out_row_stride, int rows, int B, int max_nodes, int max_ctx,
+                    int H, int Hkv, int Dh, float softmax_scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The accepted path of every tree becomes context, in all layers (layer_stride elements apart): cached row ctx_len[b] + path[b][j]
+ * moves to ctx_len[b] + j, j < min(n_accept[b], max_path), max_path <= 64; a node number outside 0 .. 63 moves nothing.  All of a
+ * request's rows are read before any is written.  len_out[b] = ctx_len[b] + n_accept[b] (not ctx_len itself; negative lengths stay). */
+int valle_paged_kv_commit(void* kcache, void* vcache, int n_layers, int64_t layer_stride, const int32_t* block_table, int max_blocks,
+                          int n_pages, int page_size, const int32_t* ctx_len, const int32_t* path, int max_path,
+                          const int32_t* n_accept, int32_t* len_out, int B, int Hkv, int Dh, int dtype, void* stream);
+
+/* valle_gemm_skinny on 4-bit weights: C[M][N] = x[M][K] . W^T, W[n][k] = scales[n][k / group] * (q[n][k] - zeros[n][k / group]),
+ * group 32, 64 or 128, K % group == 0; weights are never rounded (whole-number products, scales applied to fp32 sums).  Layout in
+ * tiles of 16 columns x 128 inputs, both rounded up, scale 0 in the padding (vall-e_amd/plugins.py HipLinear4._pack):
+ *   wq [N/16][K/128][64][16 bytes]  lane l = fq * 16 + fr: column fr of the tile; word j, byte i: inputs j * 32 + fq * 8 + i (low nibble) and
+ *                                   + i + 4 (high nibble)
+ *   scales [N/16][(K/128) * (128/group)][16] in dtype, zeros the same in bytes (NULL: 8)
+ * x: row stride in elements, rows 16-byte aligned.  Epilogues STORE (+ bias), RESID (+ bias, + resid [M][ldc]), GEGLU (no bias), F32OUT. */
+int valle_linear_w4(const void* x, int64_t x_row_stride, const void* wq, const void* scales, const uint8_t* zeros, const void* bias,
+                    const void* resid, void* C, int M, int N, int K, int group, int ldc, int epilogue, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

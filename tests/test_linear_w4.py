@@ -1,0 +1,186 @@
+"""HipLinear4 / valle_linear_w4 (vall_e_amd/plugins.py, csrc/linear_w4.hip) against the definition in 64 bits.
+
+Tolerance: the products x q are exact in fp32 (8-bit x 4-bit significands) for bf16 inputs and off by u32 = 2^-24 for fp32 ones; sums of K terms
+and the per-group scale and subtraction add (K + 32) u32 of A = sum |x| scale (q + zero); the result is rounded once (u: bf16 2^-8,
+fp32 2^-24); bias and residual add u32 of their own sums.  GEGLU: 1.13 is the largest slope of gelu, 4e-7 bounds the error of the erf
+forms relative to |gate x up|."""
+import math
+
+import pytest
+import torch
+
+from vall_e_amd import plugins as PL
+
+gpu = pytest.mark.gpu
+U32 = 2.0 ** -24
+UNIT = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+
+
+def make(n, k, group, zeros, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8)
+    s = ((torch.rand(n, k // group, generator=g) + 0.5) / math.sqrt(k)).to(dtype)
+    z = torch.randint(0, 16, (n, k // group), generator=g, dtype=torch.uint8) if zeros else None
+    return q, s, z
+
+
+def weights(q, s, z, group):
+    n = q.shape[0]
+    w = torch.stack((q & 15, q >> 4), -1).reshape(n, -1).double()
+    zz = torch.full_like(s, 8).double() if z is None else z.double()
+    zz, ss = zz.repeat_interleave(group, 1), s.double().repeat_interleave(group, 1)
+    return (w - zz) * ss, (w + zz) * ss
+
+
+def expect(x, q, s, z, group, bias=None, resid=None, geglu=False):
+    w, a = weights(q, s, z, group)
+    x = x.double()
+    y, A = x @ w.T, x.abs() @ a.T
+    err = (x.shape[-1] + 32) * U32 * A
+    for t in (bias, resid):
+        if t is not None:
+            y = y + t.double()
+            err = err + 2 * U32 * (y.abs() + t.double().abs())
+    if geglu:
+        g, u, eg, eu = y[..., 0::2], y[..., 1::2], err[..., 0::2], err[..., 1::2]
+        y = torch.nn.functional.gelu(g) * u
+        err = 1.13 * eg * (u.abs() + eu) + torch.nn.functional.gelu(g).abs() * eu + 4e-7 * (g * u).abs()
+    return y, err
+
+
+def check(got, want, err, dtype):
+    e = (got.cpu().double() - want).abs()
+    lim = err + UNIT[dtype] * want.abs()
+    assert (e <= lim).all(), (float((e - lim).max()), float(e.max()))
+
+
+def test_quantize_w4_is_within_half_a_step():
+    g = torch.Generator().manual_seed(0)
+    w = torch.randn(24, 256, generator=g)
+    w[3], w[4, :64] = 0.0, w[4, :64].abs()
+    for sym in (False, True):
+        q, s, z = PL.quantize_w4(w, 64, sym)
+        assert q.dtype == torch.uint8 and q.shape == (24, 128) and s.shape == (24, 4) and (z is None) == sym
+        back, _ = weights(q, s, z, 64)
+        step = s.double().repeat_interleave(64, 1)
+        slack = 0.5 if sym else 1.0                     # asymmetric: the zero point is rounded too, its range clipped by up to half a step
+        assert ((back - w.double()).abs() <= slack * step * (1 + 1e-6) + 1e-9).all()
+
+
+def test_packed_layout_holds_every_weight():
+    """The documented layout, element by element."""
+    n, k, group = 18, 160, 32
+    q, s, z = make(n, k, group, True, torch.float32, 3)
+    m = PL.HipLinear4.from_quantized(q, s, z, group_size=group)
+    nib = torch.stack((q & 15, q >> 4), -1).reshape(n, k)
+    for col in range(n):
+        for kk in range(0, k, 7):
+            nt, fr, kb, r = col // 16, col % 16, kk // 128, kk % 128
+            j, fq, i = r // 32, r % 32 // 8, r % 8
+            byte = int(m.wq[nt, kb, fq * 16 + fr, j * 4 + i % 4])
+            assert (byte >> 4 if i >= 4 else byte & 15) == int(nib[col, kk])
+            assert m.scales[nt, kk // group, fr] == s[col, kk // group] and m.zeros[nt, kk // group, fr] == z[col, kk // group]
+    assert (m.scales[1, :, 2:] == 0).all() and (m.scales[:, 5:] == 0).all()
+
+
+def test_refusals_without_a_gpu():
+    from vall_e_amd import _lib as L
+    import ctypes as C
+    for kw in (dict(in_features=100), dict(in_features=96, group_size=64), dict(in_features=128, group_size=48)):
+        with pytest.raises(L.ValleHipError):
+            PL.HipLinear4(out_features=8, **kw)
+    with pytest.raises(L.ValleHipError):
+        PL.HipLinear4(64, 8)(torch.zeros(1, 64))
+    q, s, z = make(8, 64, 64, True, torch.float32, 0)
+    for a in ((q.int(), s, z), (q, s[:4], z), (q, s, z.int())):
+        with pytest.raises((ValueError, L.ValleHipError)):
+            PL.HipLinear4.from_quantized(*a)
+    lib, p = L.load(), C.c_void_p(4096)
+
+    def call(**kw):
+        a = dict(x=p, rs=128, wq=p, M=2, N=32, K=128, group=64, ldc=32, epi=0, dt=1, bias=None, resid=None)
+        a.update(kw)
+        return lib.valle_linear_w4(a["x"], a["rs"], a["wq"], p, None, a["bias"], a["resid"], p, a["M"], a["N"], a["K"], a["group"], a["ldc"], a["epi"], a["dt"], None)
+    for kw, rc in ((dict(x=None), -1), (dict(dt=5), -1), (dict(group=16), -2), (dict(K=96), -1), (dict(N=0), -1), (dict(M=-1), -1), (dict(epi=1), -1), (dict(epi=6), -1),
+                   (dict(epi=2, N=31), -1), (dict(epi=2, bias=p), -1), (dict(ldc=31), -1), (dict(x=C.c_void_p(4098)), -1), (dict(rs=127), -1)):
+        assert call(**kw) == rc, kw
+        assert b"valle_linear_w4" in lib.valle_last_error()
+    assert call(M=0) == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("rows,n,k,group", [(1, 1, 32, 32), (1, 16, 128, 64), (2, 40, 96, 32), (16, 33, 256, 128), (17, 64, 160, 32), (5, 1000, 1024, 64), (64, 48, 448, 64),
+                                            (65, 100, 384, 128), (3, 256, 4096, 128), (150, 24, 256, 32), (33, 512, 2048, 64)])
+def test_linear_w4(gpu_device, dtype, zeros, rows, n, k, group):
+    q, s, z = make(n, k, group, zeros, dtype, rows + n)
+    g = torch.Generator().manual_seed(k)
+    x = torch.randn(rows, k, generator=g).to(dtype)
+    bias, resid = torch.randn(n, generator=g).to(dtype), torch.randn(rows, n, generator=g).to(dtype)
+    d = lambda t: None if t is None else t.to(gpu_device)
+    m = PL.HipLinear4.from_quantized(d(q), d(s), d(z), group_size=group)
+    check(m(d(x)), *expect(x, q, s, z, group), dtype)
+    check(m(d(x), resid=d(resid)), *expect(x, q, s, z, group, resid=resid), dtype)
+    if n % 2 == 0:
+        check(m(d(x), geglu=True), *expect(x, q, s, z, group, geglu=True), dtype)
+    mb = PL.HipLinear4.from_quantized(d(q), d(s), d(z), group_size=group, bias=d(bias))
+    check(mb(d(x)), *expect(x, q, s, z, group, bias=bias), dtype)
+
+
+@gpu
+def test_linear_w4_shapes_views_and_rows_of_others(gpu_device):
+    """Leading dimensions, strided and misaligned inputs, no rows; an infinity or NaN in one row stays in that row."""
+    n, k, group = 72, 320, 64
+    q, s, z = make(n, k, group, True, torch.bfloat16, 9)
+    d = lambda t: t.to(gpu_device)
+    m = PL.HipLinear4.from_quantized(d(q), d(s), d(z), group_size=group)
+    big = torch.randn(24, 2 * k + 8, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(gpu_device)
+    x = big[:, 8:8 + k]
+    want, err = expect(x.cpu(), q, s, z, group)
+    check(m(x), want, err, torch.bfloat16)
+    off = big[:, 3:3 + k]
+    check(m(off), *expect(off.cpu(), q, s, z, group), torch.bfloat16)
+    y = m(x.reshape(2, 3, 4, k))
+    assert y.shape == (2, 3, 4, n) and torch.equal(y.reshape(24, n), m(x))
+    assert m(x[0]).shape == (n,) and torch.equal(m(x[0]), m(x)[0])
+    assert m(x[:0]).shape == (0, n)
+    bad = x.clone()
+    bad[5, 7], bad[9, 0] = float("nan"), float("inf")
+    got = m(bad)
+    keep = [i for i in range(24) if i not in (5, 9)]
+    assert torch.equal(got[keep], m(x)[keep]) and torch.isnan(got[5]).all() and not torch.isfinite(got[9]).any()
+    for exc, kw in ((TypeError, dict(x=x.float())), (ValueError, dict(x=x[:, :64])), (ValueError, dict(x=x, resid=x)), (ValueError, dict(x=x, geglu=True, resid=x))):
+        with pytest.raises(exc):
+            m(**kw)
+
+
+@gpu
+def test_linear_w4_rows_do_not_depend_on_their_neighbours(gpu_device):
+    """A row's result is the same bits alone, in a batch of 16 and in one of 64 (every output sums its k blocks in one order)."""
+    for dtype in (torch.bfloat16, torch.float32):
+        q, s, z = make(64, 1024, 64, True, dtype, 2)
+        d = lambda t: t.to(gpu_device)
+        m = PL.HipLinear4.from_quantized(d(q), d(s), d(z))
+        x = torch.randn(100, 1024, generator=torch.Generator().manual_seed(3)).to(dtype).to(gpu_device)
+        full = m(x)
+        for rows in (1, 16, 40):
+            assert torch.equal(m(x[:rows]), full[:rows]), rows
+
+
+@gpu
+def test_linear_w4_replaces_nn_linear(gpu_device):
+    """klass of replace_linear: constructed like nn.Linear, filled from the replaced module's state dict."""
+    torch.manual_seed(0)
+    lin = torch.nn.Linear(256, 96).to(gpu_device, torch.float32)
+    m = PL.HipLinear4(256, 96, bias=True, device=gpu_device, dtype=torch.float32)
+    m.load_state_dict(lin.state_dict())
+    same = PL.HipLinear4.from_linear(lin)
+    x = torch.randn(2, 7, 256, device=gpu_device)
+    assert torch.equal(m(x), same(x))
+    q, s, z = PL.quantize_w4(lin.weight.cpu())
+    check(m(x), *expect(x.cpu(), q, s, z, 64, bias=lin.bias.detach().cpu()), torch.float32)
+    assert (m(x) - lin(x)).abs().max() < 0.5 * lin(x).abs().max()                       # 4 bits: near, not equal
+    again = PL.HipLinear4(256, 96, bias=True, device=gpu_device, dtype=torch.float32)
+    again.load_state_dict(m.state_dict())                                               # its own state dict, packed
+    assert torch.equal(again(x), m(x))

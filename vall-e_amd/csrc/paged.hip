@@ -1,0 +1,415 @@
+// The bookkeeping and the data movement of a paged KV cache: pages of `page_size` rows (a power of two), per layer
+// [n_pages][Hkv][page_size][64], a head's keys in one page contiguous as in the slot cache of valle_rope_kv.
+//   valle_page_plan          block tables, slot map, positions and tree masks from the requests' lengths
+//   valle_rope_kv_paged      RoPE on q and k rows, k and v into the pages the slot map names
+//   valle_paged_kv_commit    the accepted path of a draft tree to the end of the context, all layers
+// The reference has no counterpart: it recomputes the whole sequence per step (models/base.py:521, use_cache=False).
+#include "common.h"
+
+// ------------------------------------------------------------------------------------ page plan
+// need_b = ceil(len_new_b / page), held_b = pages in hand.  held > need: the surplus goes back on the free stack; held < need:
+// the difference comes off it, in request order, until it runs dry.  With F = free pages after all returns and x the running
+// number of a page over all requests, both are one formula: page x <-> free_list[F - 1 - x] (taking the same pages back and
+// forth leaves the stack as it was).
+#define PLAN_MAX_B 4096
+struct PlanArgs {
+    const int32_t *len_old, *len_new;
+    int32_t* table;
+    const int32_t* nb_in; int32_t* nb_out;
+    int32_t* free_list;
+    const int32_t* fc_in; int32_t* fc_out;
+    int32_t *status, *cu, *slots, *pos;
+    const int32_t* parents; int64_t* mask;
+    int B, width, n_pages, shift, max_rows;
+};
+
+__device__ __forceinline__ long plan_wave_scan(long v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long t = __shfl_up(v, o, 64);
+        if (lane >= o) v += t;
+    }
+    return v;
+}
+// exclusive prefix of v over the workgroup's threads, and the total
+template <int NT>
+__device__ __forceinline__ long plan_block_scan(long v, long* tmp, long& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long inc = plan_wave_scan(v, lane);
+    __syncthreads();
+    if (lane == 63) tmp[wave] = inc;
+    __syncthreads();
+    long base = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+        const long t = tmp[w];
+        if (w < wave) base += t;
+        sum += t;
+    }
+    total = sum;
+    return base + inc - v;
+}
+// first b in [0, B) with incl[b] > x (the caller knows that there is one)
+__device__ __forceinline__ int plan_find(const int* incl, int B, int x) {
+    int lo = 0, hi = B - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (incl[mid] > x) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+}
+__device__ __forceinline__ int plan_slot(const PlanArgs& a, int b, int p, bool served) {
+    if (!served) return -1;
+    const int blk = p >> a.shift;                              // served: len_new <= width << shift, so blk < width
+    const int page = a.table[(size_t)b * a.width + blk];
+    return page >= 0 && page < a.n_pages ? (page << a.shift) + (p & ((1 << a.shift) - 1)) : -1;
+}
+// plain rows: row r belongs to the request whose end lies behind it; rows behind the last request are padding (slot -1)
+__device__ __forceinline__ void plan_row(const PlanArgs& a, const int* ends, const int* stat, int r) {
+    if (r >= ends[a.B - 1]) { a.slots[r] = -1; a.pos[r] = 0; return; }
+    const int b = plan_find(ends, a.B, r);
+    const int p = a.len_old[b] + r - (b ? ends[b - 1] : 0);
+    a.slots[r] = plan_slot(a, b, p, stat[b] == 0);
+    a.pos[r] = p;
+}
+// tree rows of one request: lane i = node i.  Ancestor bits and depths by pointer doubling (6 rounds cover 64 levels).
+__device__ __forceinline__ void plan_tree(const PlanArgs& a, int b, int start, int n, bool served, int lane) {
+    int up = -1;
+    if (lane < n && start + lane < a.max_rows) {
+        const int p = a.parents[start + lane];
+        if (p >= 0 && p < lane) up = p;
+    }
+    uint64_t m = 1ull << lane;
+    int depth = up >= 0;
+#pragma unroll
+    for (int it = 0; it < 6; ++it) {
+        const int src = up >= 0 ? up : lane;
+        const uint32_t lo = __shfl((uint32_t)m, src, 64), hi = __shfl((uint32_t)(m >> 32), src, 64);
+        const int d = __shfl(depth, src, 64), u = __shfl(up, src, 64);
+        if (up >= 0) { m |= ((uint64_t)hi << 32) | lo; depth += d; up = u; }
+    }
+    const int r = start + lane;
+    if (lane < n && r < a.max_rows) {
+        a.slots[r] = plan_slot(a, b, a.len_old[b] + lane, served);
+        a.pos[r] = a.len_old[b] + depth;
+        a.mask[r] = (int64_t)m;
+    }
+}
+
+// One workgroup plans the batch (a request per thread, up to four); ROWS: it also fills the rows, else page_rows_kernel does.
+template <int NT, bool ROWS>
+__global__ __launch_bounds__(NT) void page_plan_kernel(PlanArgs a) {
+    constexpr int E = 4;
+    __shared__ int s_f[NT * E], s_a[NT * E], s_held[NT * E], s_end[NT * E];
+    __shared__ long tmp[NT / 64];
+    const int tid = threadIdx.x, per = (a.B + NT - 1) / NT, b0 = tid * per;
+    const long cap = (long)a.width << a.shift;
+    const int fc = min(max(*a.fc_in, 0), a.n_pages);
+    int held[E], want[E], rows[E];
+    bool ok[E], valid[E];
+    long sum = 0, total;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        held[e] = want[e] = rows[e] = 0; ok[e] = valid[e] = false;
+        const int b = b0 + e;
+        if (e < per && b < a.B) {
+            const int lo = a.len_old[b], ln = a.len_new[b];
+            held[e] = a.nb_in[b];
+            valid[e] = lo >= 0 && ln >= 0 && lo <= cap && ln <= cap && held[e] >= 0 && held[e] <= a.width && !(a.parents && ln - lo > 64);
+            want[e] = valid[e] ? (int)(((long)ln + (1 << a.shift) - 1) >> a.shift) : 0;
+            rows[e] = valid[e] && ln > lo ? ln - lo : 0;
+        }
+        sum += rows[e];
+    }
+    long at = plan_block_scan<NT>(sum, tmp, total);
+    long moved = 0;                                            // (pages given back) << 32 | pages asked for
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int b = b0 + e;
+        if (e < per && b < a.B) {
+            if (b == 0) a.cu[0] = 0;
+            at += rows[e];
+            const int end = (int)min(at, (long)INT32_MAX);
+            a.cu[b + 1] = end; s_end[b] = end;
+            ok[e] = valid[e] && at <= a.max_rows;
+            if (ok[e]) moved += ((long)max(held[e] - want[e], 0) << 32) + max(want[e] - held[e], 0);
+        }
+    }
+    long pre = plan_block_scan<NT>(moved, tmp, total);
+    const int freed = (int)(total >> 32), F = fc + freed;      // (B * width is bounded on the host: both halves stay below 2^31)
+    int f = (int)(pre >> 32), q = (int)(pre & 0xffffffff), taken = 0;
+    int stat[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int b = b0 + e;
+        stat[e] = 0;
+        if (e < per && b < a.B) {
+            const int back = ok[e] ? max(held[e] - want[e], 0) : 0, need = ok[e] ? max(want[e] - held[e], 0) : 0;
+            f += back; q += need;
+            s_f[b] = f; s_a[b] = q; s_held[b] = held[e];
+            const bool served = ok[e] && (need == 0 || q <= F);
+            if (served && need) taken = q;                     // q ascends: the last served one is the largest
+            stat[e] = !valid[e] ? 2 : !ok[e] ? 3 : served ? 0 : 1;
+            a.status[b] = stat[e];
+            a.nb_out[b] = served ? want[e] : held[e];
+        }
+    }
+    // the number of pages taken: maximum over the threads
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) taken = max(taken, __shfl_xor(taken, o, 64));
+    __syncthreads();
+    if ((tid & 63) == 0) tmp[tid >> 6] = taken;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) taken = max(taken, (int)tmp[w]);
+    if (tid == 0) *a.fc_out = F - taken;
+    for (int x = tid; x < freed; x += NT) {
+        const int b = plan_find(s_f, a.B, x), p0 = b ? s_f[b - 1] : 0;
+        const int j = s_held[b] - (s_f[b] - p0) + x - p0, dst = F - 1 - x;
+        if (dst >= 0 && dst < a.n_pages) a.free_list[dst] = a.table[(size_t)b * a.width + j];
+    }
+    __syncthreads();
+    for (int x = tid; x < taken; x += NT) {
+        const int b = plan_find(s_a, a.B, x), p0 = b ? s_a[b - 1] : 0, src = F - 1 - x;
+        a.table[(size_t)b * a.width + s_held[b] + x - p0] = src < a.n_pages ? a.free_list[src] : -1;
+    }
+    if constexpr (ROWS) {
+        __syncthreads();                                       // the tables are whole, s_f is free
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (e < per && b0 + e < a.B) s_f[b0 + e] = stat[e];
+        __syncthreads();
+        if (a.parents) {
+            for (int b = tid >> 6; b < a.B; b += NT / 64) {
+                const int start = b ? s_end[b - 1] : 0;
+                plan_tree(a, b, start, s_end[b] - start, s_f[b] == 0, tid & 63);
+            }
+            for (int r = s_end[a.B - 1] + tid; r < a.max_rows; r += NT) { a.slots[r] = -1; a.pos[r] = 0; a.mask[r] = 0; }
+        } else {
+            for (int r = tid; r < a.max_rows; r += NT) plan_row(a, s_end, s_f, r);
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void page_rows_kernel(PlanArgs a) {
+    __shared__ int s_end[PLAN_MAX_B], s_stat[PLAN_MAX_B];
+    for (int b = threadIdx.x; b < a.B; b += 256) { s_end[b] = a.cu[b + 1]; s_stat[b] = a.status[b]; }
+    __syncthreads();
+    if (a.parents) {
+        for (int b = blockIdx.x * 4 + (threadIdx.x >> 6); b < a.B; b += gridDim.x * 4) {
+            const int start = b ? s_end[b - 1] : 0;
+            plan_tree(a, b, start, s_end[b] - start, s_stat[b] == 0, threadIdx.x & 63);
+        }
+        for (long r = (long)s_end[a.B - 1] + blockIdx.x * 256 + threadIdx.x; r < a.max_rows; r += gridDim.x * 256) {
+            a.slots[r] = -1; a.pos[r] = 0; a.mask[r] = 0;
+        }
+    } else {
+        for (long r = (long)blockIdx.x * 256 + threadIdx.x; r < a.max_rows; r += gridDim.x * 256) plan_row(a, s_end, s_stat, (int)r);
+    }
+}
+
+static int page_shift(int page_size) {
+    for (int s = 4; s <= 8; ++s)
+        if (page_size == 1 << s) return s;
+    return -1;
+}
+
+extern "C" int valle_page_plan(const int32_t* len_old, const int32_t* len_new, int B, int page_size, int32_t* block_table, int max_blocks,
+                               const int32_t* n_blocks_in, int32_t* n_blocks_out, int32_t* free_list, int n_pages,
+                               const int32_t* free_count_in, int32_t* free_count_out, int32_t* status, int32_t* cu_rows,
+                               int32_t* slots, int32_t* positions, int max_rows, const int32_t* parents, int64_t* tree_mask, void* stream) {
+    VALLE_REQUIRE(len_old && len_new && block_table && n_blocks_in && n_blocks_out && free_list && free_count_in && free_count_out && status && cu_rows &&
+                  slots && positions, VALLE_E_ARG, "valle_page_plan: null pointer");
+    VALLE_REQUIRE(B > 0 && B <= PLAN_MAX_B, VALLE_E_ARG, "valle_page_plan: %d requests (1 .. %d)", B, PLAN_MAX_B);
+    const int shift = page_shift(page_size);
+    VALLE_REQUIRE(shift > 0, VALLE_E_ARG, "valle_page_plan: page_size %d (16, 32, 64, 128 or 256)", page_size);
+    VALLE_REQUIRE(max_blocks > 0 && (int64_t)B * max_blocks <= INT32_MAX && ((int64_t)max_blocks << shift) <= INT32_MAX, VALLE_E_ARG,
+                  "valle_page_plan: max_blocks %d", max_blocks);
+    VALLE_REQUIRE(n_pages > 0 && ((int64_t)n_pages << shift) <= INT32_MAX, VALLE_E_ARG, "valle_page_plan: n_pages %d", n_pages);
+    VALLE_REQUIRE(max_rows > 0, VALLE_E_ARG, "valle_page_plan: max_rows %d", max_rows);
+    VALLE_REQUIRE((parents == nullptr) == (tree_mask == nullptr), VALLE_E_ARG, "valle_page_plan: parents and tree_mask go together");
+    PlanArgs a{len_old, len_new, block_table, n_blocks_in, n_blocks_out, free_list, free_count_in, free_count_out, status, cu_rows, slots, positions,
+               parents, tree_mask, B, max_blocks, n_pages, shift, max_rows};
+    hipStream_t s = (hipStream_t)stream;
+    if (max_rows <= 4096) {
+        page_plan_kernel<1024, true><<<1, 1024, 0, s>>>(a);
+    } else {
+        page_plan_kernel<1024, false><<<1, 1024, 0, s>>>(a);
+        page_rows_kernel<<<min(ceil_div(max_rows, 256), 1024), 256, 0, s>>>(a);
+    }
+    VALLE_LAUNCH_CHECK();
+    return VALLE_OK;
+}
+
+// ------------------------------------------------------------------------------------ RoPE + write into pages
+// Elements (2i, 2i + 1) of a q or k head rotate by rope[position][i] = (cos, sin), products and sums in fp32, one rounding at
+// the end (valle_rope_kv rounds cos and sin to bf16 first, as the reference's cast tables are; here the table stays fp32: the
+// result is the formula's within one rounding).  Memory-bound: 2 x 64 x es bytes per head and row.
+struct RopePagedArgs {
+    const void *q, *k, *v; void* qo;
+    const int32_t* pos; const float* rope; const int32_t* slots;
+    void *kc, *vc;
+    long q_rs, k_rs, v_rs, qo_rs;       // row strides, elements
+    long n_slots;
+    int rope_rows, H, Hkv, shift;
+};
+
+template <typename T>
+__device__ __forceinline__ void rope_turn(const uint4& in, const float4* cs, uint4& out) {
+    constexpr int V = 16 / sizeof(T);
+    typedef T vec_t __attribute__((ext_vector_type(V)));
+    const vec_t x = __builtin_bit_cast(vec_t, in);
+    vec_t y;
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {                          // two pairs per float4 of the table
+        const float4 t = cs[i];
+        const float a0 = to_f32<T>(x[4 * i]), b0 = to_f32<T>(x[4 * i + 1]), a1 = to_f32<T>(x[4 * i + 2]), b1 = to_f32<T>(x[4 * i + 3]);
+        y[4 * i] = from_f32<T>(a0 * t.x - b0 * t.y); y[4 * i + 1] = from_f32<T>(b0 * t.x + a0 * t.y);
+        y[4 * i + 2] = from_f32<T>(a1 * t.z - b1 * t.w); y[4 * i + 3] = from_f32<T>(b1 * t.z + a1 * t.w);
+    }
+    out = __builtin_bit_cast(uint4, y);
+}
+
+// One row per workgroup of 128 threads: a thread owns one 16-byte piece of the head and walks the heads, so it reads its
+// piece of the table once.
+template <typename T>
+__global__ __launch_bounds__(128) void rope_kv_paged_kernel(RopePagedArgs a) {
+    constexpr int V = 16 / sizeof(T), CH = 64 / V, HS = 128 / CH;       // elements and pieces per head, heads at a time
+    const long r = blockIdx.x;
+    const int c = threadIdx.x % CH, h0 = threadIdx.x / CH;
+    const int slot = a.slots ? a.slots[r] : -1;
+    const int p = min(max(a.pos[r], 0), a.rope_rows - 1);
+    float4 cs[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) cs[i] = *reinterpret_cast<const float4*>(a.rope + (long)p * 64 + c * V + 4 * i);
+    if (a.q) {
+        const T* q = (const T*)a.q + r * a.q_rs + c * V;
+        T* o = (T*)a.qo + r * a.qo_rs + c * V;
+        for (int h = h0; h < a.H; h += HS) {
+            const uint4 x = *reinterpret_cast<const uint4*>(q + h * 64);
+            uint4 y;
+            rope_turn<T>(x, cs, y);
+            *reinterpret_cast<uint4*>(o + h * 64) = y;
+        }
+    }
+    if (slot < 0 || slot >= a.n_slots) return;                          // padding, a refused request: nothing is cached
+    const long page = slot >> a.shift, off = slot & ((1 << a.shift) - 1);
+    const T* k = (const T*)a.k + r * a.k_rs + c * V;
+    const T* v = (const T*)a.v + r * a.v_rs + c * V;
+    for (int h = h0; h < a.Hkv; h += HS) {
+        const uint4 x = *reinterpret_cast<const uint4*>(k + h * 64);
+        const uint4 w = *reinterpret_cast<const uint4*>(v + h * 64);
+        uint4 y;
+        rope_turn<T>(x, cs, y);
+        const long at = (((page * a.Hkv + h) << a.shift) + off) * 64 + c * V;
+        *reinterpret_cast<uint4*>((T*)a.kc + at) = y;
+        *reinterpret_cast<uint4*>((T*)a.vc + at) = w;
+    }
+}
+
+extern "C" int valle_rope_kv_paged(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride,
+                                   void* q_out, int64_t q_out_row_stride, const int32_t* positions, const float* rope, int rope_rows,
+                                   const int32_t* slots, int M, int H, int Hkv, int Dh, void* kcache, void* vcache, int n_pages, int page_size,
+                                   int dtype, void* stream) {
+    VALLE_REQUIRE(k && v && positions && rope && slots && kcache && vcache, VALLE_E_ARG, "valle_rope_kv_paged: null pointer");
+    VALLE_REQUIRE((q == nullptr) == (q_out == nullptr), VALLE_E_ARG, "valle_rope_kv_paged: q and q_out go together");
+    VALLE_REQUIRE(dtype == VALLE_BF16 || dtype == VALLE_F32, VALLE_E_ARG, "valle_rope_kv_paged: unknown dtype %d", dtype);
+    VALLE_REQUIRE(Dh == 64, VALLE_E_UNSUPPORTED, "valle_rope_kv_paged: head_dim %d (64 is built)", Dh);
+    VALLE_REQUIRE(M >= 0 && H > 0 && Hkv > 0 && rope_rows > 0, VALLE_E_ARG, "valle_rope_kv_paged: M=%d H=%d Hkv=%d rope_rows=%d", M, H, Hkv, rope_rows);
+    const int shift = page_shift(page_size);
+    VALLE_REQUIRE(shift > 0, VALLE_E_ARG, "valle_rope_kv_paged: page_size %d (16, 32, 64, 128 or 256)", page_size);
+    VALLE_REQUIRE(n_pages > 0 && ((int64_t)n_pages << shift) <= INT32_MAX, VALLE_E_ARG, "valle_rope_kv_paged: n_pages %d", n_pages);
+    const int vec = 16 / (int)dtype_size(dtype);
+    const void* ptrs[] = {q, k, v, q_out, rope, kcache, vcache};
+    for (const void* p : ptrs) VALLE_REQUIRE(((uintptr_t)p & 15) == 0, VALLE_E_ARG, "valle_rope_kv_paged: tensors must be 16-byte aligned");
+    const int64_t strides[] = {q ? q_row_stride : 0, k_row_stride, v_row_stride, q ? q_out_row_stride : 0};
+    for (int64_t st : strides) VALLE_REQUIRE(st % vec == 0 && st >= 0, VALLE_E_ARG, "valle_rope_kv_paged: row strides must keep rows 16-byte aligned");
+    VALLE_REQUIRE(!q || M <= 1 || q_out_row_stride >= (int64_t)H * 64, VALLE_E_ARG, "valle_rope_kv_paged: rows of q_out overlap");
+    if (M == 0) return VALLE_OK;
+    RopePagedArgs a{q, k, v, q_out, positions, rope, slots, kcache, vcache, q_row_stride, k_row_stride, v_row_stride, q_out_row_stride,
+                    (long)n_pages << shift, rope_rows, H, Hkv, shift};
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == VALLE_BF16) rope_kv_paged_kernel<bf16><<<M, 128, 0, s>>>(a);
+    else rope_kv_paged_kernel<float><<<M, 128, 0, s>>>(a);
+    VALLE_LAUNCH_CHECK();
+    return VALLE_OK;
+}
+
+// ------------------------------------------------------------------------------------ commit of an accepted path
+// cache[layer][ctx + j] = cache[layer][ctx + path[j]], j < n_accept.  Source and destination ranges overlap: a workgroup reads
+// every row it moves of one (request, head, layer) into registers, meets at a barrier, and writes.
+struct CommitArgs {
+    void *kc, *vc;
+    const int32_t *table, *ctx, *path, *n_accept;
+    int32_t* len_out;
+    long layer_stride;                  // elements
+    int width, max_path, n_pages, shift, Hkv;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void kv_commit_kernel(CommitArgs a) {
+    constexpr int V = 16 / sizeof(T), CH = 64 / V, TPI = 256 / (2 * CH), IT = 64 / TPI;   // pieces per row, rows at a time, rounds
+    const int h = blockIdx.x, b = blockIdx.y;
+    const long layer = blockIdx.z;
+    const int ctx = a.ctx[b];
+    const int n = min(max(a.n_accept[b], 0), a.max_path);
+    if (h == 0 && layer == 0 && threadIdx.x == 0) a.len_out[b] = ctx < 0 ? ctx : ctx + n;
+    if (ctx < 0 || n == 0) return;
+    const int c = threadIdx.x % CH, isv = (threadIdx.x / CH) & 1, t0 = threadIdx.x / (2 * CH);
+    T* cache = (T*)(isv ? a.vc : a.kc) + layer * a.layer_stride;
+    const int32_t* tab = a.table + (long)b * a.width;
+    const long cap = (long)a.width << a.shift;
+    auto place = [&](long p) -> long {                                  // element offset of cached row p, -1: not in the cache
+        if (p >= cap) return -1;
+        const int page = tab[p >> a.shift];
+        if (page < 0 || page >= a.n_pages) return -1;
+        return ((((long)page * a.Hkv + h) << a.shift) + (p & ((1 << a.shift) - 1))) * 64 + c * V;
+    };
+    uint4 x[IT];
+    long dst[IT];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        const int j = i * TPI + t0;
+        x[i] = uint4{0, 0, 0, 0}; dst[i] = -1;
+        if (j < n) {
+            const int from = a.path[(long)b * a.max_path + j];
+            if (from >= 0 && from < 64 && from != j) {
+                const long src = place((long)ctx + from);
+                if (src >= 0) {
+                    x[i] = *reinterpret_cast<const uint4*>(cache + src);
+                    dst[i] = place((long)ctx + j);
+                }
+            }
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                    // the rows are in registers before any of them is written over
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+        if (dst[i] >= 0) *reinterpret_cast<uint4*>(cache + dst[i]) = x[i];
+}
+
+extern "C" int valle_paged_kv_commit(void* kcache, void* vcache, int n_layers, int64_t layer_stride, const int32_t* block_table, int max_blocks,
+                                     int n_pages, int page_size, const int32_t* ctx_len, const int32_t* path, int max_path,
+                                     const int32_t* n_accept, int32_t* len_out, int B, int Hkv, int Dh, int dtype, void* stream) {
+    VALLE_REQUIRE(kcache && vcache && block_table && ctx_len && path && n_accept && len_out, VALLE_E_ARG, "valle_paged_kv_commit: null pointer");
+    VALLE_REQUIRE(len_out != ctx_len, VALLE_E_ARG, "valle_paged_kv_commit: len_out must not be ctx_len (every workgroup reads the lengths)");
+    VALLE_REQUIRE(dtype == VALLE_BF16 || dtype == VALLE_F32, VALLE_E_ARG, "valle_paged_kv_commit: unknown dtype %d", dtype);
+    VALLE_REQUIRE(Dh == 64, VALLE_E_UNSUPPORTED, "valle_paged_kv_commit: head_dim %d (64 is built)", Dh);
+    VALLE_REQUIRE(B >= 0 && B <= 65535 && n_layers > 0 && n_layers <= 65535 && Hkv > 0 && max_blocks > 0, VALLE_E_ARG,
+                  "valle_paged_kv_commit: B=%d n_layers=%d Hkv=%d max_blocks=%d", B, n_layers, Hkv, max_blocks);
+    VALLE_REQUIRE(max_path > 0 && max_path <= 64, VALLE_E_ARG, "valle_paged_kv_commit: max_path %d (1 .. 64)", max_path);
+    const int shift = page_shift(page_size);
+    VALLE_REQUIRE(shift > 0, VALLE_E_ARG, "valle_paged_kv_commit: page_size %d (16, 32, 64, 128 or 256)", page_size);
+    VALLE_REQUIRE(n_pages > 0 && ((int64_t)n_pages << shift) <= INT32_MAX, VALLE_E_ARG, "valle_paged_kv_commit: n_pages %d", n_pages);
+    VALLE_REQUIRE(n_layers == 1 || layer_stride >= ((int64_t)n_pages << shift) * Hkv * 64, VALLE_E_ARG, "valle_paged_kv_commit: layers overlap");
+    VALLE_REQUIRE((((uintptr_t)kcache | (uintptr_t)vcache) & 15) == 0 && layer_stride % 8 == 0, VALLE_E_ARG, "valle_paged_kv_commit: caches must be 16-byte aligned");
+    if (B == 0) return VALLE_OK;
+    CommitArgs a{kcache, vcache, block_table, ctx_len, path, n_accept, len_out, layer_stride, max_blocks, max_path, n_pages, shift, Hkv};
+    dim3 grid(Hkv, B, n_layers);
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == VALLE_BF16) kv_commit_kernel<bf16><<<grid, 256, 0, s>>>(a);
+    else kv_commit_kernel<float><<<grid, 256, 0, s>>>(a);
+    VALLE_LAUNCH_CHECK();
+    return VALLE_OK;
+}

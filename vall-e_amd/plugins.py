@@ -5,18 +5,25 @@
   vall_e/models/arch/llama.py:396-403; registered through ``AVAILABLE_ATTENTIONS``,
   vall_e/models/arch/attention/__init__.py:11-198).
 * ``HipLinear`` is a module for ``ml.replace_linear(model, klass)`` (vall_e/utils/utils.py:364-462,
-  applied in ``load_engines`` under ``cfg.optimizations.replace``, vall_e/engines/__init__.py:95-100).
+  applied in ``load_engines`` under ``cfg.optimizations.replace``, vall_e/engines/__init__.py:95-100); ``HipLinear4`` is the same
+  with 4-bit weights and group scales, for decode steps.
 
 Both call libvalle_hip.so through ctypes; tensors stay torch tensors (torch is the allocator and stream carrier).
 Inference only: no autograd."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 
 import torch
 
 from . import _lib as L
+
+
+def _device_of(t):
+    """The tensor's device as the current one (no context switch when it is that already)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
 
 
 def _strides3(t):
@@ -83,6 +90,122 @@ class HipLinear(torch.nn.Module):
             L.check(L.load().valle_gemm(L.ptr(x2), L.ptr(w.contiguous()), L.ptr(self.bias), None, L.ptr(out), M, N, self.in_features, N,
                                         L.EPI_STORE, L.dtype_code(x.dtype), L.stream_ptr(x.device)))
         return out.reshape(*x.shape[:-1], N)
+
+
+def quantize_w4(weight, group_size=64, symmetric=False):
+    """4-bit weights by groups of ``group_size`` along the input: ``(q, scales, zeros)`` with ``w ~ scales * (q - zeros)``, q uint8
+    ``[out][in / 2]`` (two to a byte, the even input in the low nibble), scales ``[out][in / group]`` in the weight's type, zeros
+    uint8 of the same shape (None when symmetric: 8)."""
+    n, k = weight.shape
+    w = weight.detach().float().reshape(n, k // group_size, group_size)
+    if symmetric:
+        s = (w.abs().amax(-1) / 7.0).to(weight.dtype).float()
+        z = torch.full_like(s, 8.0)
+    else:
+        lo, hi = w.amin(-1).clamp(max=0.0), w.amax(-1).clamp(min=0.0)
+        s = ((hi - lo) / 15.0).to(weight.dtype).float()
+        z = torch.where(s > 0, (-lo / s.clamp(min=torch.finfo(torch.float32).tiny)).round().clamp(0, 15), torch.zeros_like(s))
+    d = torch.where(s > 0, s, torch.ones_like(s))
+    q = (w / d[..., None] + z[..., None]).round().clamp(0, 15).to(torch.uint8).reshape(n, k)
+    return q[:, 0::2] | (q[:, 1::2] << 4), s.to(weight.dtype), None if symmetric else z.to(torch.uint8)
+
+
+class HipLinear4(torch.nn.Module):
+    """``nn.Linear`` with 4-bit weights and group scales on ``valle_linear_w4``, for the few rows of a decode step (any number is
+    right; from some hundred on a product on unpacked weights is the better choice): ``klass`` for the reference's
+    ``replace_linear`` -- constructed as ``klass(in_features, out_features, bias=...)``, a state dict that holds ``weight`` is
+    quantised while it loads (vall_e/utils/utils.py:400-428).  ``from_linear`` quantises a module, ``from_quantized`` takes
+    ``quantize_w4``'s layout.  ``forward(x, resid=None, geglu=False)``: + bias, + resid, or gelu(even columns) * odd columns."""
+
+    GROUPS = (32, 64, 128)
+
+    def __init__(self, in_features, out_features, bias=True, device=None, dtype=None, group_size=64, symmetric=False):
+        super().__init__()
+        if group_size not in self.GROUPS or in_features % group_size or in_features <= 0 or out_features <= 0:
+            raise L.ValleHipError(f"HipLinear4: group_size one of {self.GROUPS} that divides in_features (got {group_size}, {in_features})")
+        dtype = dtype or torch.get_default_dtype()
+        L.dtype_code(dtype)
+        self.in_features, self.out_features, self.group_size, self.symmetric = in_features, out_features, group_size, symmetric
+        nt, kb, gpb = -(-out_features // 16), -(-in_features // 128), 128 // group_size
+        self.register_buffer("wq", torch.zeros((nt, kb, 64, 16), dtype=torch.uint8, device=device))
+        self.register_buffer("scales", torch.zeros((nt, kb * gpb, 16), dtype=dtype, device=device))
+        self.register_buffer("zeros", None if symmetric else torch.zeros((nt, kb * gpb, 16), dtype=torch.uint8, device=device))
+        self.bias = torch.nn.Parameter(torch.zeros(out_features, device=device, dtype=dtype), requires_grad=False) if bias else None
+
+    @torch.no_grad()
+    def _pack(self, q, scales, zeros):
+        n, k, (nt, kb) = self.out_features, self.in_features, self.wq.shape[:2]
+        dev = self.wq.device
+        nib = torch.zeros((nt * 16, kb * 128), dtype=torch.uint8, device=dev)
+        q = q.to(dev)
+        nib[:n, 0:k:2], nib[:n, 1:k:2] = q & 15, q >> 4
+        t = nib.view(nt, 16, kb, 4, 4, 8).permute(0, 2, 4, 1, 3, 5)                          # tile, k block, fq, fr, word, weight
+        self.wq.copy_((t[..., :4] | (t[..., 4:] << 4)).reshape(nt, kb, 64, 16))
+
+        def tiles(m, fill, like):
+            p = torch.full((nt * 16, like.shape[1]), fill, dtype=like.dtype, device=dev)
+            p[:n, :k // self.group_size] = m.to(dev, like.dtype)
+            like.copy_(p.view(nt, 16, -1).transpose(1, 2))
+        tiles(scales, 0, self.scales)
+        if self.zeros is not None:
+            tiles(zeros, 0, self.zeros)
+
+    @classmethod
+    def from_quantized(cls, q, scales, zeros=None, group_size=64, bias=None):
+        m = cls(q.shape[1] * 2, q.shape[0], bias=bias is not None, device=q.device, dtype=scales.dtype, group_size=group_size, symmetric=zeros is None)
+        shape = (m.out_features, m.in_features // group_size)
+        if q.dtype is not torch.uint8 or tuple(scales.shape) != shape or (zeros is not None and (zeros.dtype is not torch.uint8 or tuple(zeros.shape) != shape)):
+            raise ValueError(f"HipLinear4: q uint8 (out, in / 2), scales and uint8 zeros {shape} needed")
+        m._pack(q, scales, zeros)
+        if bias is not None:
+            with torch.no_grad():
+                m.bias.copy_(bias)
+        return m
+
+    @classmethod
+    def from_linear(cls, lin: torch.nn.Linear, group_size=64, symmetric=False):
+        q, s, z = quantize_w4(lin.weight, group_size, symmetric)
+        return cls.from_quantized(q, s, z, group_size=group_size, bias=lin.bias.detach() if lin.bias is not None else None)
+
+    def _load_from_state_dict(self, state_dict, prefix, *args, **kw):
+        w = state_dict.pop(prefix + "weight", None)
+        if w is not None:
+            if tuple(w.shape) != (self.out_features, self.in_features):
+                raise ValueError(f"HipLinear4: weight {tuple(w.shape)} for ({self.out_features}, {self.in_features})")
+            self._pack(*quantize_w4(w.to(self.scales.dtype), self.group_size, self.symmetric))
+            state_dict.update({prefix + n: b for n, b in self.named_buffers(recurse=False)})
+        super()._load_from_state_dict(state_dict, prefix, *args, **kw)
+
+    def forward(self, x, resid=None, geglu=False):
+        s = self.scales
+        if not x.is_cuda:
+            raise L.ValleHipError("HipLinear4 needs GPU tensors; there is no CPU fallback")
+        if x.dtype is not s.dtype or x.device != s.device:
+            raise TypeError(f"HipLinear4: input {x.dtype} on {x.device}, scales {s.dtype} on {s.device}")
+        K, N = self.in_features, self.out_features
+        if x.shape[-1] != K:
+            raise ValueError(f"HipLinear4: input of width {x.shape[-1]}, {K} needed")
+        n_out, epi, bias = N, L.EPI_STORE, self.bias
+        if geglu:
+            if resid is not None or bias is not None or N % 2:
+                raise ValueError("HipLinear4: geglu takes an even number of columns, no bias and no residual")
+            n_out, epi = N // 2, L.EPI_GEGLU
+        x2 = x if x.dim() == 2 and x.stride(1) == 1 else x.reshape(-1, K)
+        if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.data_ptr() % 16:
+            x2 = x2.clone(memory_format=torch.contiguous_format)
+        M = x2.shape[0]
+        out = torch.empty((*x.shape[:-1], n_out), dtype=x.dtype, device=x.device)
+        if resid is not None:
+            if resid.shape != out.shape or resid.dtype is not x.dtype or resid.device != x.device:
+                raise ValueError(f"HipLinear4: residual {tuple(resid.shape)} {resid.dtype} for {tuple(out.shape)} {x.dtype}")
+            resid, epi = resid.contiguous(), L.EPI_RESID
+        if M:
+            with _device_of(x):
+                L.check(L.load().valle_linear_w4(x2.data_ptr(), x2.stride(0), self.wq.data_ptr(), s.data_ptr(),
+                                                 None if self.zeros is None else self.zeros.data_ptr(), None if bias is None else bias.data_ptr(),
+                                                 None if resid is None else resid.data_ptr(), out.data_ptr(), M, N, K, self.group_size, n_out, epi,
+                                                 L.dtype_code(x.dtype), L.stream_ptr(x.device)))
+        return out
 
 
 class HipEmbedding(torch.nn.Module):
