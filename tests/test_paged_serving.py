@@ -644,6 +644,19 @@ def test_kv_commit_layer_slices_and_counts_out_of_range(gpu_device):
     assert torch.equal(kc, k0)
 
 
+@gpu
+def test_empty_calls(gpu_device):
+    """No rows, no requests: nothing to do, nothing touched."""
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=gpu_device)
+    kc, vc = randn((1, 3, 2, 16, 64), torch.float32, 1, gpu_device), randn((1, 3, 2, 16, 64), torch.float32, 2, gpu_device)
+    k0 = kc.clone()
+    q = torch.zeros(0, 2, 64, device=gpu_device)
+    assert P.rope_kv_paged(q, q, q, i32(0), rope_table(4).to(gpu_device), i32(0), kc[0], vc[0]).shape == (0, 2, 64)
+    assert P.attn_tree(q, kc[0], vc[0], i32(2, 1), i32(2), i32(3)).shape == (0, 2, 64)
+    assert P.attn_tree(torch.zeros(3, 2, 64, device=gpu_device), kc[0], vc[0], i32(0, 1), i32(0), i32(1)).shape == (3, 2, 64)
+    assert P.kv_commit(kc, vc, i32(0, 1), i32(0), i32(0, 2), i32(0)).shape == (0,) and torch.equal(kc, k0)
+
+
 # --------------------------------------------------------------------------------------- refusals that need a device
 @gpu
 def test_gpu_refusals(gpu_device):

@@ -81,6 +81,21 @@ template <typename T> __device__ __forceinline__ float gelu_act(float x) {
     else return gelu_erf(x);
 }
 
+// Bounds-checked loads through a buffer descriptor: a lane whose offset lies at or behind `bytes` gets zeros and moves no data, and
+// the load is issued either way -- a loop's prefetch past its end stays countable (a load that may not have been issued makes the
+// compiler wait for everything under way) and costs nothing.  The descriptor is wave-uniform; offsets are 32-bit.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buf_rsrc(const void* base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
+#define BUF_OFF 0x80000000u     // an offset behind every descriptor (descriptors are kept below 2^31 bytes)
+__device__ __forceinline__ uint4 buf_load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+}
+__device__ __forceinline__ uint2 buf_load8(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+}
+__device__ __forceinline__ uint32_t buf_load4(__amdgpu_buffer_rsrc_t r, uint32_t off) { return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0); }
+
 static inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 static inline size_t align_up(size_t a, size_t b) { return (a + b - 1) / b * b; }
 static inline size_t dtype_size(int dtype) { return dtype == VALLE_BF16 ? 2 : 4; }

@@ -25,6 +25,11 @@ __device__ __forceinline__ bf16x8 w4_fragment(uint32_t w) {
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+__device__ __forceinline__ uint32_t w4_word(const uint4& w, int j) { return j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w; }
+__device__ __forceinline__ float w4_value(uint32_t w, int i) {           // weight i of a word: v_cvt_f32_ubyte of one byte
+    return (float)((((i < 4 ? w : w >> 4) & 0x0f0f0f0fu) >> ((i & 3) * 8)) & 255u);
+}
+
 template <typename T>
 __device__ __forceinline__ void w4_store(const W4Args& a, int m, int n, const f32x4& v) {          // columns n .. n + 3 of row m
     if (m >= a.M) return;
@@ -51,89 +56,260 @@ __device__ __forceinline__ void w4_store(const W4Args& a, int m, int n, const f3
     }
 }
 
-// One workgroup: 16 output columns x up to 16 * MT rows; its waves split the k blocks, partial sums meet in LDS in wave order.
-template <typename T, int G, int MT, int NW>
+// ---- the bf16 form.  A wave owns NT column tiles x MT row tiles and every NW-th k block; the loads of the next one are under way
+// while one is multiplied (two more under way: slower, 10.0 against 9.3 us at 8192 -> 8192).  Partial sums of the waves meet in LDS, in wave order.
+template <int GPB, int NT, int MT> struct W4Stage { uint4 w[NT]; uint2 s[GPB][NT]; uint32_t z[GPB][NT]; uint4 x[MT][4]; };
+
+template <int G, int NT, int MT, int NW>
 __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
     constexpr int GPB = 128 / G, FPG = G / 32;                           // groups per k block, fragments per group
-    const int nt = blockIdx.x, m0 = blockIdx.y * 16 * MT;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
-    const uint4* wp = a.wq + (long)nt * a.KB * 64 + lane;
-    const T* sp = (const T*)a.scales + (long)nt * a.KB * GPB * 16 + fq * 4;
-    const uint8_t* zp = a.zeros ? a.zeros + (long)nt * a.KB * GPB * 16 + fq * 4 : nullptr;
-    f32x4 acc[MT];
+    const int nt0 = blockIdx.x * NT, m0 = blockIdx.y * 16 * MT, tiles = (a.N + 15) >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
+    __shared__ f32x4 lds[NW * (NT > 4 ? NT : 4) * MT * 64];              // x of the waves, then their partial sums
+    // x is loaded four lanes to a row (64 bytes in a piece; a row per lane, as the fragments have it, runs at a quarter of the rate)
+    // and turned to fragment order through the wave's own LDS; the rotation by 4 pieces per column keeps both sides free of conflicts.
+    uint4* xl = reinterpret_cast<uint4*>(lds) + wave * MT * 4 * 64;
+    const int xw = (lane & 3) * 16 + (((lane >> 2) + 4 * (lane & 3)) & 15), xr = fq * 16 + ((fr + 4 * fq) & 15);
+    const int rows = min(a.M - m0, 16 * MT);
+    const __amdgpu_buffer_rsrc_t xb = buf_rsrc((const bf16*)a.x + (long)m0 * a.x_rs, (uint32_t)(((rows - 1) * a.x_rs + a.K) * 2));
+    uint32_t xo[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int kb = wave; kb < a.KB; kb += NW) {
-        const uint4 w4 = wp[(long)kb * 64];
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+    for (int t = 0; t < MT; ++t) xo[t] = (uint32_t)(min(t * 16 + (lane >> 2), rows - 1) * a.x_rs + (lane & 3) * 8) * 2;   // rows behind the last: never stored
+    __amdgpu_buffer_rsrc_t wb[NT], sb[NT], zb[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {                                       // tiles behind the last one read zeros
+        const long nt = nt0 + n;
+        const bool on = nt < tiles;
+        wb[n] = buf_rsrc(a.wq + nt * a.KB * 64, on ? a.KB * 1024 : 0);
+        sb[n] = buf_rsrc((const bf16*)a.scales + nt * a.KB * GPB * 16, on ? a.KB * GPB * 32 : 0);
+        zb[n] = buf_rsrc(a.zeros + nt * a.KB * GPB * 16, on && a.zeros ? a.KB * GPB * 16 : 0);
+    }
+    const bool has_z = a.zeros != nullptr;
+    typedef W4Stage<GPB, NT, MT> Stage;
+    auto load = [&](Stage& st, int kb) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            st.w[n] = buf_load16(wb[n], kb * 1024 + lane * 16);
+#pragma unroll
+            for (int g = 0; g < GPB; ++g) {
+                st.s[g][n] = buf_load8(sb[n], (kb * GPB + g) * 32 + fq * 8);
+                st.z[g][n] = buf_load4(zb[n], (kb * GPB + g) * 16 + fq * 4);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = kb * 128 + j * 32;                             // K % 32 == 0: a fragment is in or out as a whole
+#pragma unroll
+            for (int t = 0; t < MT; ++t) st.x[t][j] = buf_load16(xb, k < a.K ? xo[t] + k * 2 : BUF_OFF);
+        }
+    };
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto use = [&](const Stage& st) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) xl[(j * MT + t) * 64 + xw] = st.x[t][j];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int g = 0; g < GPB; ++g) {
-            typedef T vec4 __attribute__((ext_vector_type(4)));
-            const vec4 sv = *reinterpret_cast<const vec4*>(sp + (long)(kb * GPB + g) * 16);
-            const uint32_t zv = zp ? *reinterpret_cast<const uint32_t*>(zp + (long)(kb * GPB + g) * 16) : 0x08080808u;
-            f32x4 xq[MT], xs[MT];
+            f32x4 xq[NT][MT], xs[MT];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) xq[t] = xs[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; t < MT; ++t) {
+                xs[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) xq[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
 #pragma unroll
             for (int f = 0; f < FPG; ++f) {
-                const int j = g * FPG + f, k = kb * 128 + j * 32 + fq * 8;
+                const int j = g * FPG + f;
+                if constexpr (MT == 3) __builtin_amdgcn_sched_barrier(0);
+                const bf16 one = (bf16)1.0f;
+                bf16x8 x[MT];
 #pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    const int m = m0 + t * 16 + fr;
-                    const bool in = m < a.M && k < a.K;                  // K % 32 == 0: a lane's 8 are in or out together
-                    const T* xp = (const T*)a.x + (long)m * a.x_rs + k;
-                    if constexpr (sizeof(T) == 2) {
-                        bf16x8 xv = {};
-                        if (in) xv = *reinterpret_cast<const bf16x8*>(xp);
-                        const bf16 one = (bf16)1.0f;
-                        xq[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w4_fragment(w[j]), xv, xq[t], 0, 0, 0);
-                        xs[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16x8{one, one, one, one, one, one, one, one}, xv, xs[t], 0, 0, 0);
-                    } else {
-                        f32x4 x0 = {0.f, 0.f, 0.f, 0.f}, x1 = x0;
-                        if (in) { x0 = *reinterpret_cast<const f32x4*>(xp); x1 = *reinterpret_cast<const f32x4*>(xp + 4); }
+                for (int t = 0; t < MT; ++t) x[t] = __builtin_bit_cast(bf16x8, xl[(j * MT + t) * 64 + xr]);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float qv = (float)((w[j] >> ((i & 3) * 8 + (i >> 2) * 4)) & 15u), xv = i < 4 ? x0[i & 3] : x1[i & 3];
-                            xq[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(qv, xv, xq[t], 0, 0, 0);
-                            xs[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(1.0f, xv, xs[t], 0, 0, 0);
-                        }
-                    }
+                for (int t = 0; t < MT; ++t)
+                    xs[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16x8{one, one, one, one, one, one, one, one}, x[t], xs[t], 0, 0, 0);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const bf16x8 q = w4_fragment(w4_word(st.w[n], j));
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) xq[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q, x[t], xq[n][t], 0, 0, 0);
                 }
             }
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+            for (int n = 0; n < NT; ++n) {
+                const bf16x4 sv = __builtin_bit_cast(bf16x4, st.s[g][n]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[t][r] += to_f32<T>(sv[r]) * (xq[t][r] - (float)((zv >> (8 * r)) & 255u) * xs[t][r]);
+                for (int r = 0; r < 4; ++r) {
+                    const float s = (float)sv[r], z = has_z ? (float)((st.z[g][n] >> (8 * r)) & 255u) : 8.0f;
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) acc[n][t][r] = fmaf(s, fmaf(-z, xs[t][r], xq[n][t][r]), acc[n][t][r]);
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    Stage st[2];
+    load(st[0], wave);
+    for (int kb = wave; kb < a.KB; kb += 2 * NW) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (kb + u * NW >= a.KB) break;
+            load(st[1 - u], kb + (u + 1) * NW);
+            __builtin_amdgcn_sched_barrier(0);                           // (left alone the compiler sinks the loads behind the products)
+            use(st[u]);
         }
     }
-    __shared__ f32x4 part[NW][MT][64];
+    typedef f32x4 part_t[NT * MT][64];
+    part_t* part = reinterpret_cast<part_t*>(lds);
+    __syncthreads();                                                     // every wave is done with its x
 #pragma unroll
-    for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) part[wave][n * MT + t][lane] = acc[n][t];
+    __syncthreads();
+    for (int i = threadIdx.x; i < NT * MT * 64; i += NW * 64) {
+        const int p = i >> 6, l = i & 63, n = p / MT, t = p % MT;
+        f32x4 s = part[0][p][l];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) {
+            const f32x4 v = part[w][p][l];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[r] += v[r];
+        }
+        w4_store<bf16>(a, m0 + t * 16 + (l & 15), (nt0 + n) * 16 + (l >> 4) * 4, s);
+    }
+}
+
+// ---- the fp32 form: weights become (q - zero) * scale in fp32 (one rounding), the group structure ends there; an MFMA takes 4 inputs, the
+// k slots of a fragment are dealt so that a lane's 8 weights of a word meet its 8 values of x.  Two accumulators, for the dependent chain.
+template <int GPB, int MT> struct W4Stage32 { uint4 w; float s[GPB]; uint32_t z[GPB]; uint4 x[MT][8]; };
+
+template <int G, int MT, int NW>
+__global__ __launch_bounds__(NW * 64) void linear_w4_f32_kernel(W4Args a) {
+    constexpr int GPB = 128 / G;
+    const int m0 = blockIdx.y * 16 * MT;
+    const long nt = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
+    __shared__ f32x4 lds[NW * MT * 8 * 64];                              // x of the waves, then their partial sums
+    uint4* xl = reinterpret_cast<uint4*>(lds) + wave * MT * 8 * 64;
+    const int pc = lane & 3, rw = lane >> 2;                             // this lane loads pieces pc and pc + 4 (of 8 per fragment) of row rw
+    const int rows = min(a.M - m0, 16 * MT);
+    const __amdgpu_buffer_rsrc_t xb = buf_rsrc((const float*)a.x + (long)m0 * a.x_rs, (uint32_t)(((rows - 1) * a.x_rs + a.K) * 4));
+    uint32_t xo[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xo[t] = (uint32_t)(min(t * 16 + rw, rows - 1) * a.x_rs + pc * 4) * 4;
+    const __amdgpu_buffer_rsrc_t wb = buf_rsrc(a.wq + nt * a.KB * 64, a.KB * 1024);
+    const __amdgpu_buffer_rsrc_t sb = buf_rsrc((const float*)a.scales + nt * a.KB * GPB * 16, a.KB * GPB * 64);
+    const __amdgpu_buffer_rsrc_t zb = buf_rsrc(a.zeros + nt * a.KB * GPB * 16, a.zeros ? a.KB * GPB * 16 : 0);
+    const bool has_z = a.zeros != nullptr;
+    typedef W4Stage32<GPB, MT> Stage;
+    auto load = [&](Stage& st, int kb) {
+        st.w = buf_load16(wb, kb * 1024 + lane * 16);
+#pragma unroll
+        for (int g = 0; g < GPB; ++g) {
+            st.s[g] = __builtin_bit_cast(float, buf_load4(sb, (kb * GPB + g) * 64 + fr * 4));
+            st.z[g] = buf_load4(zb, (kb * GPB + g) * 16 + (fr & 12));
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int k = kb * 128 + (j >> 1) * 32;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) st.x[t][j] = buf_load16(xb, k < a.K ? xo[t] + kb * 512 + j * 64 : BUF_OFF);
+        }
+    };
+    f32x4 acc[2][MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[0][t] = acc[1][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto use = [&](const Stage& st) {
+        // piece p (of 8) of row r at p * 16 + (r + 4 p) % 16: both sides free of bank conflicts
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) xl[((j >> 1) * MT + t) * 128 + ((j & 1) * 4 + pc) * 16 + ((rw + 4 * pc) & 15)] = st.x[t][j];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int g = j * 32 / G;
+            const float z = has_z ? (float)((st.z[g] >> ((fr & 3) * 8)) & 255u) : 8.0f;
+            f32x4 x[MT][2];
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) x[t][e] = __builtin_bit_cast(f32x4, xl[(j * MT + t) * 128 + (2 * fq + e) * 16 + ((fr + 8 * fq + 4 * e) & 15)]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float w = (w4_value(w4_word(st.w, j), i) - z) * st.s[g];
+#pragma unroll
+                for (int t = 0; t < MT; ++t) acc[i & 1][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, x[t][i >> 2][i & 3], acc[i & 1][t], 0, 0, 0);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    Stage st[2];
+    load(st[0], wave);
+    for (int kb = wave; kb < a.KB; kb += 2 * NW) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (kb + u * NW >= a.KB) break;
+            load(st[1 - u], kb + (u + 1) * NW);
+            __builtin_amdgcn_sched_barrier(0);
+            use(st[u]);
+        }
+    }
+    typedef f32x4 part_t[MT][64];
+    part_t* part = reinterpret_cast<part_t*>(lds);
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < MT; ++t) part[wave][t][lane] = f32x4{acc[0][t][0] + acc[1][t][0], acc[0][t][1] + acc[1][t][1], acc[0][t][2] + acc[1][t][2], acc[0][t][3] + acc[1][t][3]};
     __syncthreads();
     for (int i = threadIdx.x; i < MT * 64; i += NW * 64) {
         const int t = i >> 6, l = i & 63;
         f32x4 s = part[0][t][l];
 #pragma unroll
         for (int w = 1; w < NW; ++w) {
-            const f32x4 p = part[w][t][l];
+            const f32x4 v = part[w][t][l];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[r] += p[r];
+            for (int r = 0; r < 4; ++r) s[r] += v[r];
         }
-        w4_store<T>(a, m0 + t * 16 + (l & 15), nt * 16 + (l >> 4) * 4, s);
+        w4_store<float>(a, m0 + t * 16 + (l & 15), nt * 16 + (l >> 4) * 4, s);
     }
 }
 
-template <typename T, int G>
-static void w4_launch(const W4Args& a, hipStream_t s) {
-    const int nt = ceil_div(a.N, 16);
-    if (a.M <= 16) linear_w4_kernel<T, G, 1, 8><<<dim3(nt, 1), 512, 0, s>>>(a);
-    else linear_w4_kernel<T, G, 4, 8><<<dim3(nt, ceil_div(a.M, 64)), 512, 0, s>>>(a);
+// Row tiles per workgroup: the fewest (more workgroups) that keep the launch within one workgroup per CU, else equal blocks of up to `most`.
+static int w4_row_tiles(int M, int gx, int most) {
+    for (int mt = 1; mt < most; ++mt)
+        if ((long)gx * ceil_div(M, 16 * mt) <= 256) return mt;
+    return ceil_div(ceil_div(M, ceil_div(M, 16 * most)), 16);
 }
-template <typename T>
-static void w4_launch_group(const W4Args& a, int group, hipStream_t s) {
-    if (group == 32) w4_launch<T, 32>(a, s);
-    else if (group == 64) w4_launch<T, 64>(a, s);
-    else w4_launch<T, 128>(a, s);
+template <int G, int NT>
+static void w4_launch_bf16(const W4Args& a, hipStream_t s) {
+    const int gx = ceil_div(ceil_div(a.N, 16), NT), mt = w4_row_tiles(a.M, gx, 3);
+    const dim3 grid(gx, ceil_div(a.M, 16 * mt));
+    if (mt == 1) linear_w4_kernel<G, NT, 1, 8><<<grid, 512, 0, s>>>(a);
+    else if (mt == 2) linear_w4_kernel<G, NT, 2, 8><<<grid, 512, 0, s>>>(a);
+    else linear_w4_kernel<G, NT, 3, 8><<<grid, 512, 0, s>>>(a);
+}
+template <int G>
+static void w4_launch(const W4Args& a, int dtype, hipStream_t s) {
+    if (dtype == VALLE_BF16) {
+        // two column tiles per wave share the row fragments: from 256 workgroups of two tiles on, measured at 8192 -> 8192, group 128:
+        // 9.2 against 11.0 us for 1 .. 16 rows, 14.1 against 19.5 for 32; below, one (the chip would not be filled)
+        if (a.N >= 8192) w4_launch_bf16<G, 2>(a, s);
+        else w4_launch_bf16<G, 1>(a, s);
+        return;
+    }
+    // (two row tiles per workgroup take as long as two workgroups: 55.3 against 2 x 27.2 us at 8192 -> 8192; the MFMAs bound it)
+    linear_w4_f32_kernel<G, 1, 8><<<dim3(ceil_div(a.N, 16), ceil_div(a.M, 16)), 512, 0, s>>>(a);
 }
 
 extern "C" int valle_linear_w4(const void* x, int64_t x_row_stride, const void* wq, const void* scales, const uint8_t* zeros, const void* bias,
@@ -149,11 +325,15 @@ extern "C" int valle_linear_w4(const void* x, int64_t x_row_stride, const void* 
     VALLE_REQUIRE(ldc >= (epilogue == VALLE_EPI_GEGLU ? N / 2 : N), VALLE_E_ARG, "valle_linear_w4: ldc %d too small", ldc);
     VALLE_REQUIRE((((uintptr_t)x | (uintptr_t)wq | (uintptr_t)scales | (uintptr_t)zeros) & 15) == 0, VALLE_E_ARG, "valle_linear_w4: operands must be 16-byte aligned");
     VALLE_REQUIRE(x_row_stride >= 0 && x_row_stride % (16 / (int)dtype_size(dtype)) == 0, VALLE_E_ARG, "valle_linear_w4: rows of x must stay 16-byte aligned");
-    VALLE_REQUIRE(M <= 65535 * 64, VALLE_E_ARG, "valle_linear_w4: %d rows", M);
+    VALLE_REQUIRE(x_row_stride <= 1 << 23 && (int64_t)ceil_div(K, 128) * 1024 <= INT32_MAX / 2, VALLE_E_ARG, "valle_linear_w4: x_row_stride %lld or K %d too large",
+                  (long long)x_row_stride, K);
+    VALLE_REQUIRE(M <= 65535 * 16, VALLE_E_ARG, "valle_linear_w4: %d rows", M);
     if (M == 0) return VALLE_OK;
     W4Args a{x, (const uint4*)wq, scales, zeros, bias, resid, C, x_row_stride, M, N, K, ceil_div(K, 128), ldc, epilogue};
-    if (dtype == VALLE_BF16) w4_launch_group<bf16>(a, group, (hipStream_t)stream);
-    else w4_launch_group<float>(a, group, (hipStream_t)stream);
+    hipStream_t st = (hipStream_t)stream;
+    if (group == 32) w4_launch<32>(a, dtype, st);
+    else if (group == 64) w4_launch<64>(a, dtype, st);
+    else w4_launch<128>(a, dtype, st);
     VALLE_LAUNCH_CHECK();
     return VALLE_OK;
 }

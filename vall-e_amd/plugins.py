@@ -12,18 +12,12 @@ Both call libvalle_hip.so through ctypes; tensors stay torch tensors (torch is t
 Inference only: no autograd."""
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import math
 
 import torch
 
 from . import _lib as L
-
-
-def _device_of(t):
-    """The tensor's device as the current one (no context switch when it is that already)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
 
 
 def _strides3(t):
@@ -130,7 +124,7 @@ class HipLinear4(torch.nn.Module):
         self.register_buffer("wq", torch.zeros((nt, kb, 64, 16), dtype=torch.uint8, device=device))
         self.register_buffer("scales", torch.zeros((nt, kb * gpb, 16), dtype=dtype, device=device))
         self.register_buffer("zeros", None if symmetric else torch.zeros((nt, kb * gpb, 16), dtype=torch.uint8, device=device))
-        self.bias = torch.nn.Parameter(torch.zeros(out_features, device=device, dtype=dtype), requires_grad=False) if bias else None
+        self.register_parameter("bias", torch.nn.Parameter(torch.zeros(out_features, device=device, dtype=dtype), requires_grad=False) if bias else None)
 
     @torch.no_grad()
     def _pack(self, q, scales, zeros):
@@ -177,34 +171,40 @@ class HipLinear4(torch.nn.Module):
         super()._load_from_state_dict(state_dict, prefix, *args, **kw)
 
     def forward(self, x, resid=None, geglu=False):
-        s = self.scales
-        if not x.is_cuda:
+        bufs, dev = self._buffers, x.get_device()          # (the dictionaries: a module's attribute lookup takes 0.4 us each)
+        wq, s, zeros, bias = bufs["wq"], bufs["scales"], bufs["zeros"], self._parameters["bias"]
+        if dev < 0:
             raise L.ValleHipError("HipLinear4 needs GPU tensors; there is no CPU fallback")
-        if x.dtype is not s.dtype or x.device != s.device:
+        if x.dtype is not s.dtype or s.get_device() != dev:
             raise TypeError(f"HipLinear4: input {x.dtype} on {x.device}, scales {s.dtype} on {s.device}")
-        K, N = self.in_features, self.out_features
-        if x.shape[-1] != K:
-            raise ValueError(f"HipLinear4: input of width {x.shape[-1]}, {K} needed")
-        n_out, epi, bias = N, L.EPI_STORE, self.bias
+        K, N, shape = self.in_features, self.out_features, x.shape
+        if shape[-1] != K:
+            raise ValueError(f"HipLinear4: input of width {shape[-1]}, {K} needed")
+        n_out, epi = N, L.EPI_STORE
         if geglu:
             if resid is not None or bias is not None or N % 2:
                 raise ValueError("HipLinear4: geglu takes an even number of columns, no bias and no residual")
             n_out, epi = N // 2, L.EPI_GEGLU
-        x2 = x if x.dim() == 2 and x.stride(1) == 1 else x.reshape(-1, K)
-        if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.data_ptr() % 16:
-            x2 = x2.clone(memory_format=torch.contiguous_format)
-        M = x2.shape[0]
-        out = torch.empty((*x.shape[:-1], n_out), dtype=x.dtype, device=x.device)
+        x2 = x if len(shape) == 2 else x.reshape(-1, K)
+        rs, step = x2.stride()
+        if step != 1 or rs % 8 or rs > 1 << 23 or x2.data_ptr() % 16:
+            x2, rs = x2.clone(memory_format=torch.contiguous_format), K
+        out = x.new_empty((*shape[:-1], n_out))
         if resid is not None:
-            if resid.shape != out.shape or resid.dtype is not x.dtype or resid.device != x.device:
+            if resid.shape != out.shape or resid.dtype is not x.dtype or resid.get_device() != dev:
                 raise ValueError(f"HipLinear4: residual {tuple(resid.shape)} {resid.dtype} for {tuple(out.shape)} {x.dtype}")
             resid, epi = resid.contiguous(), L.EPI_RESID
-        if M:
-            with _device_of(x):
-                L.check(L.load().valle_linear_w4(x2.data_ptr(), x2.stride(0), self.wq.data_ptr(), s.data_ptr(),
-                                                 None if self.zeros is None else self.zeros.data_ptr(), None if bias is None else bias.data_ptr(),
-                                                 None if resid is None else resid.data_ptr(), out.data_ptr(), M, N, K, self.group_size, n_out, epi,
-                                                 L.dtype_code(x.dtype), L.stream_ptr(x.device)))
+        if not len(x2):
+            return out
+        args = (x2.data_ptr(), rs, wq.data_ptr(), s.data_ptr(), None if zeros is None else zeros.data_ptr(), None if bias is None else bias.data_ptr(),
+                None if resid is None else resid.data_ptr(), out.data_ptr(), len(x2), N, K, self.group_size, n_out, epi, L.dtype_code(x.dtype))
+        if torch.cuda.current_device() == dev:
+            rc = L.load().valle_linear_w4(*args, L.raw_stream(dev))
+        else:
+            with torch.cuda.device(dev):
+                rc = L.load().valle_linear_w4(*args, L.raw_stream(dev))
+        if rc:
+            L.check(rc)
         return out
 
 
