@@ -23,41 +23,30 @@ struct TreeArgs {
 #define TREE_MAX_NODES 64
 #define TREE_MAX_SPLIT 64
 
-// one tile of a wave: SUB sub-tiles of 16 keys in fragment order
-template <typename T> struct TreeTile;
-template <> struct TreeTile<bf16> {
-    static constexpr int SUB = 2;
-    uint4 k[2][2];                      // key fr, dims fq * 8 .. + 8 of either half
-    uint2 v[2][4];                      // key fq * 4 + r, dims fr * 4 .. + 4
+// one tile of a wave: SUB sub-tiles of 16 keys (32 keys of bf16, 16 of fp32: 4 KB of K, 4 KB of V)
+template <typename T> struct TreeTile {
+    static constexpr int SUB = 4 / sizeof(T);
+    typedef T vrow __attribute__((ext_vector_type(4)));
+    uint4 k[4];                         // the tile's K bytes as they lie: load i, lane l = bytes i * 1024 + l * 16
+    vrow v[SUB][4];                     // key fq * 4 + r, dims fr * 4 .. + 4
     uint32_t live;                      // bit s: the page of sub-tile s is one of the cache's
 };
-template <> struct TreeTile<float> {
-    static constexpr int SUB = 1;
-    f32x4 k[1][4];                      // key fr, dims fq * 16 + 4 i .. + 4
-    f32x4 v[1][4];                      // key fq * 4 + r, dims fr * 4 .. + 4
-    uint32_t live;
-};
-
-__device__ __forceinline__ void tree_load_sub(TreeTile<bf16>& t, int s, const bf16* kp, const bf16* vp, int fr, int fq) {
-    t.k[s][0] = *reinterpret_cast<const uint4*>(kp + fr * 64 + fq * 8);
-    t.k[s][1] = *reinterpret_cast<const uint4*>(kp + fr * 64 + fq * 8 + 32);
+// K goes from the loads' order (whole 128-byte lines; a key per lane, as the fragments have it, loads at a quarter of the rate) to
+// fragment order through 4 KB of the wave's own LDS.  A row is CH pieces of 16 bytes, piece c of row r at r * CH + (c ^ (r mod CH)):
+// both sides free of bank conflicts.
+template <typename T>
+__device__ __forceinline__ void tree_stage_k(const TreeTile<T>& t, uint4* kl, int lane) {
+    constexpr int CH = 4 * (int)sizeof(T), RPL = 64 / CH;                // pieces per row, rows per load
 #pragma unroll
-    for (int r = 0; r < 4; ++r) t.v[s][r] = *reinterpret_cast<const uint2*>(vp + (fq * 4 + r) * 64 + fr * 4);
+    for (int i = 0; i < 4; ++i) {
+        const int r = i * RPL + lane / CH;
+        kl[r * CH + ((lane % CH) ^ (r % CH))] = t.k[i];
+    }
 }
-__device__ __forceinline__ void tree_load_sub(TreeTile<float>& t, int s, const float* kp, const float* vp, int fr, int fq) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t.k[s][i] = *reinterpret_cast<const f32x4*>(kp + fr * 64 + fq * 16 + i * 4);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) t.v[s][r] = *reinterpret_cast<const f32x4*>(vp + (fq * 4 + r) * 64 + fr * 4);
-}
-__device__ __forceinline__ void tree_zero_sub(TreeTile<bf16>& t, int s) {
-    t.k[s][0] = t.k[s][1] = uint4{0, 0, 0, 0};
-#pragma unroll
-    for (int r = 0; r < 4; ++r) t.v[s][r] = uint2{0, 0};
-}
-__device__ __forceinline__ void tree_zero_sub(TreeTile<float>& t, int s) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t.k[s][i] = t.v[s][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+template <typename T>
+__device__ __forceinline__ uint4 tree_k_piece(const uint4* kl, int r, int c) {
+    constexpr int CH = 4 * (int)sizeof(T);
+    return kl[r * CH + (c ^ (r % CH))];
 }
 
 template <typename T> struct TreeQuery;
@@ -71,18 +60,28 @@ __device__ __forceinline__ void tree_load_q(TreeQuery<float>& q, const float* p,
 #pragma unroll
     for (int i = 0; i < 4; ++i) q.x[i] = *reinterpret_cast<const f32x4*>(p + fq * 16 + i * 4);
 }
-__device__ __forceinline__ f32x4 tree_scores(const TreeTile<bf16>& t, int s, const TreeQuery<bf16>& q) {
-    f32x4 a = {0.f, 0.f, 0.f, 0.f};
-    a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t.k[s][0]), q.x[0], a, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t.k[s][1]), q.x[1], a, 0, 0, 0);
+// scores of sub-tile s for QB query blocks: lane = query fr, keys fq * 4 + r
+template <int QB>
+__device__ __forceinline__ void tree_scores(const uint4* kl, int s, int fr, int fq, const TreeQuery<bf16> (&q)[QB], f32x4 (&st)[QB][2]) {
+    const bf16x8 k0 = __builtin_bit_cast(bf16x8, tree_k_piece<bf16>(kl, s * 16 + fr, fq)), k1 = __builtin_bit_cast(bf16x8, tree_k_piece<bf16>(kl, s * 16 + fr, fq + 4));
+#pragma unroll
+    for (int j = 0; j < QB; ++j) {
+        st[j][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q[j].x[0], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        st[j][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q[j].x[1], st[j][s], 0, 0, 0);
+    }
 }
-__device__ __forceinline__ f32x4 tree_scores(const TreeTile<float>& t, int s, const TreeQuery<float>& q) {
-    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+template <int QB>
+__device__ __forceinline__ void tree_scores(const uint4* kl, int s, int fr, int fq, const TreeQuery<float> (&q)[QB], f32x4 (&st)[QB][1]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < QB; ++j) st[j][0] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a = __builtin_amdgcn_mfma_f32_16x16x4f32(t.k[s][i][e], q.x[i][e], a, 0, 0, 0);
-    return a;
+    for (int i = 0; i < 4; ++i) {
+        const f32x4 k = __builtin_bit_cast(f32x4, tree_k_piece<float>(kl, fr, fq * 4 + i));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int j = 0; j < QB; ++j) st[j][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], q[j].x[i][e], st[j][0], 0, 0, 0);
+    }
 }
 // o[dt] rows i = dims i * 4 + dt: the lane holds dims (fq * 4 + r) * 4 + dt of its query
 template <int QB>
@@ -98,10 +97,14 @@ __device__ __forceinline__ void tree_pv(const TreeTile<bf16>& t, const f32x4 (&p
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const uint32_t sel = dt & 1 ? 0x07060302u : 0x05040100u;
-            const uint32_t a0 = dt < 2 ? t.v[s][0].x : t.v[s][0].y, a1 = dt < 2 ? t.v[s][1].x : t.v[s][1].y;
-            const uint32_t a2 = dt < 2 ? t.v[s][2].x : t.v[s][2].y, a3 = dt < 2 ? t.v[s][3].x : t.v[s][3].y;
-            w[2 * s] = __builtin_amdgcn_perm(a1, a0, sel);
-            w[2 * s + 1] = __builtin_amdgcn_perm(a3, a2, sel);
+            uint32_t a[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint2 row = __builtin_bit_cast(uint2, t.v[s][r]);
+                a[r] = dt < 2 ? row.x : row.y;
+            }
+            w[2 * s] = __builtin_amdgcn_perm(a[1], a[0], sel);
+            w[2 * s + 1] = __builtin_amdgcn_perm(a[3], a[2], sel);
         }
         const bf16x8 vt = __builtin_bit_cast(bf16x8, uint4{w[0], w[1], w[2], w[3]});
 #pragma unroll
@@ -118,27 +121,18 @@ __device__ __forceinline__ void tree_pv(const TreeTile<float>& t, const f32x4 (&
             for (int j = 0; j < QB; ++j) o[j][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(t.v[0][r][dt], p[j][0][r], o[j][dt], 0, 0, 0);
 }
 
-// element e (0 .. 3) of a lane's V row r in sub-tile s
-__device__ __forceinline__ float tree_v(const TreeTile<bf16>& t, int s, int r, int e) {
-    const uint32_t w = e < 2 ? t.v[s][r].x : t.v[s][r].y;
-    return __builtin_bit_cast(float, e & 1 ? w & 0xffff0000u : w << 16);
-}
-__device__ __forceinline__ float tree_v(const TreeTile<float>& t, int s, int r, int e) { return t.v[s][r][e]; }
-__device__ __forceinline__ void tree_zero_v(TreeTile<bf16>& t, int s, int r) { t.v[s][r] = uint2{0, 0}; }
-__device__ __forceinline__ void tree_zero_v(TreeTile<float>& t, int s, int r) { t.v[s][r] = f32x4{0.f, 0.f, 0.f, 0.f}; }
-
-__device__ __forceinline__ void tree_clean_v(TreeTile<bf16>& t, int s, int r) {           // infinities and NaN -> 0
+template <typename T>
+__device__ __forceinline__ bool tree_odd(const TreeTile<T>& t, int s, int r) {           // infinities or NaN in the lane's 4 dims of V row r
+    bool odd = false;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        uint32_t& w = e < 2 ? t.v[s][r].x : t.v[s][r].y;
-        const uint32_t half = e & 1 ? 0xffff0000u : 0x0000ffffu;
-        if (!(fabsf(tree_v(t, s, r, e)) < INFINITY)) w &= ~half;
-    }
+    for (int e = 0; e < 4; ++e) odd |= !(fabsf(to_f32<T>(t.v[s][r][e])) < INFINITY);
+    return odd;
 }
-__device__ __forceinline__ void tree_clean_v(TreeTile<float>& t, int s, int r) {
+template <typename T>
+__device__ __forceinline__ void tree_clean_v(TreeTile<T>& t, int s, int r) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (!(fabsf(t.v[s][r][e]) < INFINITY)) t.v[s][r][e] = 0.f;
+        if (!(fabsf(to_f32<T>(t.v[s][r][e])) < INFINITY)) t.v[s][r][e] = from_f32<T>(0.f);
 }
 
 template <typename T, int QB, int NW>
@@ -182,34 +176,46 @@ __global__ __launch_bounds__(NW * 64) void attn_tree_kernel(TreeArgs a) {
     }
     __shared__ float so[NW][16][68];
     __shared__ float sm[NW][16], sl[NW][16];
-    // page of the wave's sub-tiles, 64 at a time: lane i holds sub-tile i of the current window
-    int pages = -1;
-    auto load = [&](Tile& t, int i) {                                    // tile number i of this wave
-        const int w = (i * SUB) & 63;
-        if (w == 0) {
-            const long key = (long)(t0 + wave + NW * (i + lane / SUB)) * KT + (lane % SUB) * 16;
-            pages = key < T_all ? tab[key >> a.shift] : -1;
-            if (pages >= a.n_pages) pages = -1;
-        }
+    // Every load of the loop is issued whatever the case, through bounds-checked descriptors: what lies behind the wave's last tile
+    // moves no data, and the loads stay countable.
+    const int mine = t0 + wave < t1 ? (t1 - t0 - wave + NW - 1) / NW : 0;
+    const __amdgpu_buffer_rsrc_t tb = buf_rsrc(tab, a.width * 4);
+    auto page_of = [&](int i) {                                          // lane s (mod SUB): the page of sub-tile s of this wave's tile i
+        const int key = (t0 + wave + NW * i) * KT + (lane % SUB) * 16;
+        return (int)buf_load4(tb, i < mine && key < T_all ? (uint32_t)(key >> a.shift) * 4 : BUF_OFF);
+    };
+    auto load = [&](Tile& t, int i, int pages) {
         t.live = 0;
         const int key0 = (t0 + wave + NW * i) * KT;
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
-            const int page = __builtin_amdgcn_readlane(pages, w + s);
-            if (page >= 0) {
-                const long at = page * page_stride + (long)((key0 + s * 16) & ((1 << a.shift) - 1)) * 64;
-                tree_load_sub(t, s, kbase + at, vbase + at, fr, fq);
-                t.live |= 1u << s;
-            } else tree_zero_sub(t, s);
+            const int page = __builtin_amdgcn_readlane(pages, s), key = key0 + s * 16;
+            const bool on = i < mine && key < T_all && page >= 0 && page < a.n_pages;
+            const long at = (on ? page : 0) * page_stride + (long)(key & ((1 << a.shift) - 1)) * 64;
+            const uint32_t bytes = on ? min(16, T_all - key) * 64 * (int)sizeof(T) : 0;
+            const __amdgpu_buffer_rsrc_t k = buf_rsrc(kbase + at, bytes), v = buf_rsrc(vbase + at, bytes);      // rows behind the sequence read zeros
+#pragma unroll
+            for (int i = 0; i < 4 / SUB; ++i) t.k[s * (4 / SUB) + i] = buf_load16(k, i * 1024 + lane * 16);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t off = ((fq * 4 + r) * 64 + fr * 4) * (int)sizeof(T);
+                if constexpr (sizeof(T) == 2) t.v[s][r] = __builtin_bit_cast(typename Tile::vrow, buf_load8(v, off));
+                else t.v[s][r] = __builtin_bit_cast(typename Tile::vrow, buf_load16(v, off));
+            }
+            if (on) t.live |= 1u << s;
         }
     };
     auto use = [&](Tile& t, int i) {
         const int key0 = (t0 + wave + NW * i) * KT;
+        uint4* kl = reinterpret_cast<uint4*>(&so[wave][0][0]);
+        tree_stage_k(t, kl, lane);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
         f32x4 st[QB][SUB];
 #pragma unroll
-        for (int j = 0; j < QB; ++j)
-#pragma unroll
-            for (int s = 0; s < SUB; ++s) st[j][s] = tree_scores(t, s, qf[j]);
+        for (int s = 0; s < SUB; ++s) tree_scores<QB>(kl, s, fr, fq, qf, st);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
         const bool edge = key0 + KT > ctx || t.live != (1u << SUB) - 1;  // wave-uniform: only the tiles with nodes, or with pages missing
         bool odd = false;                                                // a drafted row holds infinities or NaN
         if (edge) {
@@ -223,25 +229,40 @@ __global__ __launch_bounds__(NW * 64) void attn_tree_kernel(TreeArgs a) {
 #pragma unroll
                     for (int j = 0; j < QB; ++j)
                         if (!there || (node >= 0 && !((see[j] >> (node & 63)) & 1))) st[j][s][r] = -INFINITY;
-                    if (!there) tree_zero_v(t, s, r);                    // rows behind the sequence may hold anything (0 x NaN)
-                    else if (node >= 0) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) odd |= !(fabsf(tree_v(t, s, r, e)) < INFINITY);
-                    }
+                    if (node >= 0) odd |= tree_odd(t, s, r);             // (rows behind the sequence were read as zeros)
                 }
         }
+        // The shift of the exponentials needs to be near the maximum, not the maximum: it follows only when a score lies more than 8
+        // (a factor of 256 in a weight) above it, so that most tiles reduce nothing over lanes and scale nothing.
+        float top[QB];
+        bool grow = false;
 #pragma unroll
         for (int j = 0; j < QB; ++j) {
-            float mx = st[j][0][0];
+            top[j] = st[j][0][0];
 #pragma unroll
             for (int s = 0; s < SUB; ++s)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[j][s][r]);
-            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float mn = fmaxf(m[j], mx * a.scale_log2);             // scale > 0: the maximum commutes with it
-            const float ms = mn == -INFINITY ? 0.f : mn;                 // nothing seen so far: keep the arguments finite
-            const float alpha = __builtin_amdgcn_exp2f(m[j] - ms);
+                for (int r = 0; r < 4; ++r) top[j] = fmaxf(top[j], st[j][s][r]);
+            grow |= top[j] * a.scale_log2 > m[j] + 8.0f;                 // scale > 0: the maximum commutes with it
+        }
+        if (__any(grow)) {
+#pragma unroll
+            for (int j = 0; j < QB; ++j) {
+                float mx = fmaxf(top[j], __shfl_xor(top[j], 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float mn = mx * a.scale_log2 > m[j] + 8.0f ? mx * a.scale_log2 : m[j];      // by the query's own scores alone
+                const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[j] - mn);
+                l[j] *= alpha;
+                m[j] = mn;
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[j][dt][r] *= alpha;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < QB; ++j) {
+            const float ms = m[j] == -INFINITY ? 0.f : m[j];             // nothing seen so far: keep the arguments finite
             float sum = 0.f;
 #pragma unroll
             for (int s = 0; s < SUB; ++s)
@@ -251,12 +272,7 @@ __global__ __launch_bounds__(NW * 64) void attn_tree_kernel(TreeArgs a) {
                     st[j][s][r] = p;
                     sum += p;
                 }
-            l[j] = l[j] * alpha + sum;
-            m[j] = mn;
-#pragma unroll
-            for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[j][dt][r] *= alpha;
+            l[j] += sum;
         }
         if (edge && __any(odd)) {
             // A node's V row with infinities or NaN belongs to the queries that see it and to no other: 0 x inf in the MFMA
@@ -266,11 +282,7 @@ __global__ __launch_bounds__(NW * 64) void attn_tree_kernel(TreeArgs a) {
             for (int s = 0; s < SUB; ++s)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    bool bad = false;
-                    if (key0 + s * 16 + fq * 4 + r >= ctx) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) bad |= !(fabsf(tree_v(t, s, r, e)) < INFINITY);
-                    }
+                    const bool bad = key0 + s * 16 + fq * 4 + r >= ctx && tree_odd(t, s, r);
                     const uint64_t lanes = __ballot(bad);
 #pragma unroll
                     for (int f = 0; f < 4; ++f)
@@ -307,17 +319,22 @@ __global__ __launch_bounds__(NW * 64) void attn_tree_kernel(TreeArgs a) {
         }
         tree_pv<QB>(t, st, o);
     };
-    const int mine = t0 + wave < t1 ? (t1 - t0 - wave + NW - 1) / NW : 0;
     if (mine > 0) {
         Tile A, B;
-        load(A, 0);
-        for (int i = 0; i < mine; i += 2) {
-            if (i + 1 < mine) load(B, i + 1);
+        int next = page_of(0);
+        load(A, 0, next);
+        next = page_of(1);
+        for (int i = 0;; i += 2) {
+            int after = page_of(i + 2);
+            load(B, i + 1, next);
+            __builtin_amdgcn_sched_barrier(0);                           // (left alone the compiler sinks the loads behind the products)
             use(A, i);
-            if (i + 1 < mine) {
-                if (i + 2 < mine) load(A, i + 2);
-                use(B, i + 1);
-            }
+            if (i + 1 >= mine) break;
+            next = page_of(i + 3);
+            load(A, i + 2, after);
+            __builtin_amdgcn_sched_barrier(0);
+            use(B, i + 1);
+            if (i + 2 >= mine) break;
         }
     }
     // ---- merge of the waves, one block of 16 queries at a time
@@ -384,21 +401,28 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeArgs a) {
     const float w = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - M);
     const float L = wave_sum(w == 0.f ? 0.f : lv * w);
     float acc = 0.f;
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float ws = __shfl(w, s, 64);
-        if (ws != 0.f) acc += a.part[(at + s) * 64 + lane] * ws;
+    for (int s0 = 0; s0 < a.nsplit; s0 += 8) {                           // eight loads under way
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = a.part[(at + min(s0 + i, a.nsplit - 1)) * 64 + lane];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float ws = s0 + i < a.nsplit ? __shfl(w, (s0 + i) & 63, 64) : 0.f;
+            acc = ws == 0.f ? acc : acc + v[i] * ws;                     // (a part that saw nothing wrote no sums)
+        }
     }
     ((T*)a.out)[row * a.o_rs + head * 64 + lane] = from_f32<T>(L == 0.f ? 0.f : acc / L);
 }
 
 static int tree_qb(int nq) { return nq <= 16 ? 1 : nq <= 32 ? 2 : 4; }
-// Workgroups over the key axis: requests x kv heads x query blocks fill the chip alone from 512 on; below that the keys are
-// split until they do, as long as a wave keeps two tiles.
+// Workgroups over the key axis: requests x kv heads x query blocks fill the chip alone from 256 on; below that the keys are
+// split until they do (two workgroups of one query block share a CU, larger ones have it alone), as long as a wave keeps two tiles.
 static int tree_splits(int B, int Hkv, int g, int max_nodes, int max_ctx, int kt, int nw) {
     const int nq = max_nodes * g;
     const long base = (long)B * Hkv * ceil_div(nq, 16 * tree_qb(nq));
     const long tiles = ((long)max_ctx + max_nodes + kt - 1) / kt;
-    long s = (512 + base - 1) / base;
+    const long fill = tree_qb(nq) == 1 ? 512 : 256;
+    long s = (fill + base - 1) / base;
     if (s > tiles / (2 * nw)) s = tiles / (2 * nw);
     if (base >= 256) s = 1;
     return (int)(s < 1 ? 1 : s > TREE_MAX_SPLIT ? TREE_MAX_SPLIT : s);
@@ -437,7 +461,7 @@ extern "C" int valle_attn_tree(const void* q, int64_t q_row_stride, const void* 
     for (int i = 4; i <= 8; ++i)
         if (page_size == 1 << i) shift = i;
     VALLE_REQUIRE(shift > 0, VALLE_E_ARG, "valle_attn_tree: page_size %d (16, 32, 64, 128 or 256)", page_size);
-    VALLE_REQUIRE(n_pages > 0 && ((int64_t)n_pages << shift) <= INT32_MAX && max_blocks > 0 && ((int64_t)max_blocks << shift) <= INT32_MAX, VALLE_E_ARG,
+    VALLE_REQUIRE(n_pages > 0 && ((int64_t)n_pages << shift) <= INT32_MAX && max_blocks > 0 && ((int64_t)max_blocks << shift) <= INT32_MAX - (1 << 20), VALLE_E_ARG,
                   "valle_attn_tree: n_pages %d, max_blocks %d", n_pages, max_blocks);
     VALLE_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY, VALLE_E_ARG, "valle_attn_tree: softmax_scale must be positive");
     const int vec = 16 / (int)dtype_size(dtype);
