@@ -17,6 +17,7 @@ struct TreeArgs {
     float* part;                        // [rows * H][nsplit][64] sums, then [rows * H][nsplit][2] (maximum, denominator)
     long q_rs, o_rs;                    // elements
     float scale_log2;
+    uint32_t g_inv;                     // ceil(2^32 / g): qi / g = high word of qi * g_inv for qi < 64 g, g <= 1024
     int width, n_pages, shift, rows, H, Hkv, g, max_nodes, nsplit;
 };
 
@@ -60,37 +61,37 @@ __device__ __forceinline__ void tree_load_q(TreeQuery<float>& q, const float* p,
 #pragma unroll
     for (int i = 0; i < 4; ++i) q.x[i] = *reinterpret_cast<const f32x4*>(p + fq * 16 + i * 4);
 }
-// scores of sub-tile s for QB query blocks: lane = query fr, keys fq * 4 + r
-template <int QB>
-__device__ __forceinline__ void tree_scores(const uint4* kl, int s, int fr, int fq, const TreeQuery<bf16> (&q)[QB], f32x4 (&st)[QB][2]) {
-    const bf16x8 k0 = __builtin_bit_cast(bf16x8, tree_k_piece<bf16>(kl, s * 16 + fr, fq)), k1 = __builtin_bit_cast(bf16x8, tree_k_piece<bf16>(kl, s * 16 + fr, fq + 4));
+// K fragments of a tile out of LDS, and the scores of one query block: lane = query fr, keys fq * 4 + r of each sub-tile
+template <typename T> struct TreeKeys { uint4 x[4]; };
+__device__ __forceinline__ void tree_keys(TreeKeys<bf16>& k, const uint4* kl, int fr, int fq) {
 #pragma unroll
-    for (int j = 0; j < QB; ++j) {
-        st[j][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q[j].x[0], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-        st[j][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q[j].x[1], st[j][s], 0, 0, 0);
+    for (int s = 0; s < 2; ++s) {
+        k.x[2 * s] = tree_k_piece<bf16>(kl, s * 16 + fr, fq);
+        k.x[2 * s + 1] = tree_k_piece<bf16>(kl, s * 16 + fr, fq + 4);
     }
 }
-template <int QB>
-__device__ __forceinline__ void tree_scores(const uint4* kl, int s, int fr, int fq, const TreeQuery<float> (&q)[QB], f32x4 (&st)[QB][1]) {
+__device__ __forceinline__ void tree_keys(TreeKeys<float>& k, const uint4* kl, int fr, int fq) {
 #pragma unroll
-    for (int j = 0; j < QB; ++j) st[j][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 4; ++i) k.x[i] = tree_k_piece<float>(kl, fr, fq * 4 + i);
+}
+__device__ __forceinline__ void tree_scores(const TreeKeys<bf16>& k, const TreeQuery<bf16>& q, f32x4 (&st)[2]) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        st[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k.x[2 * s]), q.x[0], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        st[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k.x[2 * s + 1]), q.x[1], st[s], 0, 0, 0);
+    }
+}
+__device__ __forceinline__ void tree_scores(const TreeKeys<float>& k, const TreeQuery<float>& q, f32x4 (&st)[1]) {
+    st[0] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const f32x4 k = __builtin_bit_cast(f32x4, tree_k_piece<float>(kl, fr, fq * 4 + i));
+        const f32x4 kk = __builtin_bit_cast(f32x4, k.x[i]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int j = 0; j < QB; ++j) st[j][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], q[j].x[i][e], st[j][0], 0, 0, 0);
+        for (int e = 0; e < 4; ++e) st[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[e], q.x[i][e], st[0], 0, 0, 0);
     }
 }
-// o[dt] rows i = dims i * 4 + dt: the lane holds dims (fq * 4 + r) * 4 + dt of its query
-template <int QB>
-__device__ __forceinline__ void tree_pv(const TreeTile<bf16>& t, const f32x4 (&p)[QB][2], f32x4 (&o)[QB][4]) {
-    bf16x8 pf[QB];
-#pragma unroll
-    for (int j = 0; j < QB; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) pf[j][e] = (bf16)p[j][e >> 2][e & 3];      // P rounded to bf16 for the MFMA (the denominator keeps fp32)
+// V^T as the A operand.  o[dt] rows i = dims i * 4 + dt: the lane holds dims (fq * 4 + r) * 4 + dt of its query
+__device__ __forceinline__ void tree_vt(const TreeTile<bf16>& t, bf16x8 (&vt)[4]) {
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) {
         uint32_t w[4];
@@ -106,20 +107,29 @@ __device__ __forceinline__ void tree_pv(const TreeTile<bf16>& t, const f32x4 (&p
             w[2 * s] = __builtin_amdgcn_perm(a[1], a[0], sel);
             w[2 * s + 1] = __builtin_amdgcn_perm(a[3], a[2], sel);
         }
-        const bf16x8 vt = __builtin_bit_cast(bf16x8, uint4{w[0], w[1], w[2], w[3]});
-#pragma unroll
-        for (int j = 0; j < QB; ++j) o[j][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, pf[j], o[j][dt], 0, 0, 0);
+        vt[dt] = __builtin_bit_cast(bf16x8, uint4{w[0], w[1], w[2], w[3]});
     }
 }
-template <int QB>
-__device__ __forceinline__ void tree_pv(const TreeTile<float>& t, const f32x4 (&p)[QB][1], f32x4 (&o)[QB][4]) {
+__device__ __forceinline__ void tree_pv(const bf16x8 (&vt)[4], const f32x4 (&p)[2], f32x4 (&o)[4]) {
+    bf16x8 pf;
 #pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
+    for (int e = 0; e < 8; ++e) pf[e] = (bf16)p[e >> 2][e & 3];           // P rounded to bf16 for the MFMA (the denominator keeps fp32)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int j = 0; j < QB; ++j) o[j][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(t.v[0][r][dt], p[j][0][r], o[j][dt], 0, 0, 0);
+    for (int dt = 0; dt < 4; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt[dt], pf, o[dt], 0, 0, 0);
 }
+__device__ __forceinline__ void tree_vt(const TreeTile<float>& t, f32x4 (&vt)[4]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) vt[r] = t.v[0][r];
+}
+__device__ __forceinline__ void tree_pv(const f32x4 (&v)[4], const f32x4 (&p)[1], f32x4 (&o)[4]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][dt], p[0][r], o[dt], 0, 0, 0);
+}
+template <typename T> struct TreeVt;
+template <> struct TreeVt<bf16> { typedef bf16x8 type[4]; };
+template <> struct TreeVt<float> { typedef f32x4 type[4]; };
 
 template <typename T>
 __device__ __forceinline__ bool tree_odd(const TreeTile<T>& t, int s, int r) {           // infinities or NaN in the lane's 4 dims of V row r
@@ -135,19 +145,21 @@ __device__ __forceinline__ void tree_clean_v(TreeTile<T>& t, int s, int r) {
         if (!(fabsf(to_f32<T>(t.v[s][r][e])) < INFINITY)) t.v[s][r][e] = from_f32<T>(0.f);
 }
 
-template <typename T, int QB, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_tree_kernel(TreeArgs a) {
+// NQ groups of QB x 16 queries per workgroup: the waves of one key stream (there are NW / NQ) read the same tiles at about the same
+// time, so all but one of them find them in the CU's L1.
+template <typename T, int QB, int NQ, int NW>
+__global__ __launch_bounds__(NW * 64, QB == 1 && sizeof(T) == 2 ? 4 : 2) void attn_tree_kernel(TreeArgs a) {
     typedef TreeTile<T> Tile;
-    constexpr int SUB = Tile::SUB, KT = 16 * SUB;
+    constexpr int SUB = Tile::SUB, KT = 16 * SUB, NK = NW / NQ;
     const int split = blockIdx.x, kvh = blockIdx.y % a.Hkv, qblk = blockIdx.y / a.Hkv, b = blockIdx.z;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int fr = lane & 15, fq = lane >> 4;
+    const int fr = lane & 15, fq = lane >> 4, stream = wave / NQ;
     const int ctx_in = a.ctx[b], r0 = a.cu[b];
     if (ctx_in < 0 || r0 < 0) return;                                    // a finished request: its rows stay as they are
     const int nk = min(max(a.cu[b + 1] - r0, 0), TREE_MAX_NODES);        // nodes that are keys
     const int n = min(min(nk, a.max_nodes), a.rows - r0);                // nodes that ask
-    const int nq = n * a.g, q0 = qblk * 16 * QB;
-    if (n <= 0 || q0 >= nq) return;
+    const int nq = n * a.g, wg_q0 = qblk * NQ * 16 * QB, q0 = wg_q0 + wave % NQ * 16 * QB;
+    if (n <= 0 || wg_q0 >= nq) return;
     const int T_all = (int)min((long)ctx_in + nk, (long)a.width << a.shift);
     const int ctx = min(ctx_in, T_all);
     const int tiles = (T_all + KT - 1) / KT, per = (tiles + a.nsplit - 1) / a.nsplit;
@@ -157,278 +169,324 @@ __global__ __launch_bounds__(NW * 64) void attn_tree_kernel(TreeArgs a) {
     const T* kbase = (const T*)a.kc + ((long)kvh << a.shift) * 64;
     const T* vbase = (const T*)a.vc + ((long)kvh << a.shift) * 64;
     const long page_stride = ((long)a.Hkv << a.shift) * 64;
+    const uint32_t page_bytes = (uint32_t)page_stride * (uint32_t)sizeof(T);
 
+    const auto node_of = [&](int qi) { return a.g == 1 ? qi : (int)__umulhi((uint32_t)qi, a.g_inv); };    // qi / g
     TreeQuery<T> qf[QB];
     uint64_t see[QB];
 #pragma unroll
     for (int j = 0; j < QB; ++j) {
-        const int qi = min(q0 + j * 16 + fr, nq - 1), node = qi / a.g, head = kvh * a.g + qi % a.g;
+        const int qi = min(q0 + j * 16 + fr, nq - 1), node = node_of(qi), head = kvh * a.g + qi - node * a.g;
         tree_load_q(qf[j], (const T*)a.q + (long)(r0 + node) * a.q_rs + head * 64, fq);
         see[j] = a.mask ? (uint64_t)a.mask[r0 + node] : (2ull << node) - 1;
     }
-    float m[QB], l[QB];
+    float m[QB], l[QB], lim[QB], shift[QB];                              // lim: the score beyond which m follows; shift = -m (0 while nothing was seen)
     f32x4 o[QB][4];
 #pragma unroll
     for (int j = 0; j < QB; ++j) {
-        m[j] = -INFINITY; l[j] = 0.f;
+        m[j] = lim[j] = -INFINITY; l[j] = shift[j] = 0.f;
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) o[j][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    __shared__ float so[NW][16][68];
-    __shared__ float sm[NW][16], sl[NW][16];
+    __shared__ float so[QB][NW][16][68];
+    __shared__ float sm[QB][NW][16], sl[QB][NW][16];
+    __shared__ uint32_t s_odd[2];                                        // nodes whose V rows hold infinities or NaN
+    if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
+    __syncthreads();
     // Every load of the loop is issued whatever the case, through bounds-checked descriptors: what lies behind the wave's last tile
     // moves no data, and the loads stay countable.
-    const int mine = t0 + wave < t1 ? (t1 - t0 - wave + NW - 1) / NW : 0;
+    const int mine = t0 + stream < t1 && q0 < nq ? (t1 - t0 - stream + NK - 1) / NK : 0;
     const __amdgpu_buffer_rsrc_t tb = buf_rsrc(tab, a.width * 4);
     auto page_of = [&](int i) {                                          // lane s (mod SUB): the page of sub-tile s of this wave's tile i
-        const int key = (t0 + wave + NW * i) * KT + (lane % SUB) * 16;
+        const int key = (t0 + stream + NK * i) * KT + (lane % SUB) * 16;
         return (int)buf_load4(tb, i < mine && key < T_all ? (uint32_t)(key >> a.shift) * 4 : BUF_OFF);
     };
     auto load = [&](Tile& t, int i, int pages) {
         t.live = 0;
-        const int key0 = (t0 + wave + NW * i) * KT;
+        uint32_t ko = lane * 16, vo = (fq * 256 + fr * 4) * (int)sizeof(T);
+        asm("" : "+v"(ko), "+v"(vo));                                    // (kept next to the loads: their constants go into the instructions, not registers)
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
-            const int page = __builtin_amdgcn_readlane(pages, s), key = key0 + s * 16;
+            const int page = __builtin_amdgcn_readlane(pages, s), key = (t0 + stream + NK * i) * KT + s * 16;
             const bool on = i < mine && key < T_all && page >= 0 && page < a.n_pages;
-            const long at = (on ? page : 0) * page_stride + (long)(key & ((1 << a.shift) - 1)) * 64;
-            const uint32_t bytes = on ? min(16, T_all - key) * 64 * (int)sizeof(T) : 0;
-            const __amdgpu_buffer_rsrc_t k = buf_rsrc(kbase + at, bytes), v = buf_rsrc(vbase + at, bytes);      // rows behind the sequence read zeros
+            const uint64_t at = (uint64_t)(uint32_t)(on ? page : 0) * page_bytes + (uint32_t)((key & ((1 << a.shift) - 1)) * 64 * (int)sizeof(T));
+            const uint32_t bytes = on ? min(16, T_all - key) * 64 * (int)sizeof(T) : 0;      // rows behind the sequence read zeros
+            const __amdgpu_buffer_rsrc_t k = buf_rsrc((const char*)kbase + at, bytes), v = buf_rsrc((const char*)vbase + at, bytes);
 #pragma unroll
-            for (int i = 0; i < 4 / SUB; ++i) t.k[s * (4 / SUB) + i] = buf_load16(k, i * 1024 + lane * 16);
+            for (int n = 0; n < 4 / SUB; ++n) t.k[s * (4 / SUB) + n] = buf_load16(k, ko + n * 1024);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const uint32_t off = ((fq * 4 + r) * 64 + fr * 4) * (int)sizeof(T);
+                const uint32_t off = vo + r * 64 * (int)sizeof(T);
                 if constexpr (sizeof(T) == 2) t.v[s][r] = __builtin_bit_cast(typename Tile::vrow, buf_load8(v, off));
                 else t.v[s][r] = __builtin_bit_cast(typename Tile::vrow, buf_load16(v, off));
             }
             if (on) t.live |= 1u << s;
         }
     };
-    auto use = [&](Tile& t, int i) {
-        const int key0 = (t0 + wave + NW * i) * KT;
-        uint4* kl = reinterpret_cast<uint4*>(&so[wave][0][0]);
+    TreeKeys<T> kf;
+    typename TreeVt<T>::type vt;
+    uint32_t win[QB];                                                    // bit s * 16 + r: the query sees key s * 16 + fq * 4 + r of the tile
+    bool edge;
+    auto open = [&](Tile& t, int i) {                                    // the tile leaves its registers: K over LDS into fragments, V turned
+        const int key0 = (t0 + stream + NK * i) * KT;
+        uint4* kl = reinterpret_cast<uint4*>(&so[0][wave][0][0]);
         tree_stage_k(t, kl, lane);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        f32x4 st[QB][SUB];
-#pragma unroll
-        for (int s = 0; s < SUB; ++s) tree_scores<QB>(kl, s, fr, fq, qf, st);
+        tree_keys(kf, kl, fr, fq);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        const bool edge = key0 + KT > ctx || t.live != (1u << SUB) - 1;  // wave-uniform: only the tiles with nodes, or with pages missing
-        bool odd = false;                                                // a drafted row holds infinities or NaN
+        edge = key0 + KT > ctx || t.live != (1u << SUB) - 1;             // wave-uniform: only the tiles with nodes, or with pages missing
         if (edge) {
+            // A node's V row with infinities or NaN belongs to the queries that see it and to no other: 0 x inf in the MFMA would
+            // reach them all.  Such elements are taken out here and added to the seeing queries in the merge.
+            uint32_t odd = 0;
 #pragma unroll
             for (int s = 0; s < SUB; ++s)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int key = key0 + s * 16 + fq * 4 + r;
-                    const bool there = key < T_all && ((t.live >> s) & 1);
-                    const int node = key - ctx;
-#pragma unroll
-                    for (int j = 0; j < QB; ++j)
-                        if (!there || (node >= 0 && !((see[j] >> (node & 63)) & 1))) st[j][s][r] = -INFINITY;
-                    if (node >= 0) odd |= tree_odd(t, s, r);             // (rows behind the sequence were read as zeros)
+                for (int r = 0; r < 4; ++r) {                            // (rows behind the sequence were read as zeros)
+                    const bool bad = key0 + s * 16 + fq * 4 + r >= ctx && tree_odd(t, s, r);
+                    odd |= (uint32_t)bad << (s * 16 + r);
+                    if (bad) tree_clean_v(t, s, r);
                 }
-        }
-        // The shift of the exponentials needs to be near the maximum, not the maximum: it follows only when a score lies more than 8
-        // (a factor of 256 in a weight) above it, so that most tiles reduce nothing over lanes and scale nothing.
-        float top[QB];
-        bool grow = false;
+            if (__any(odd != 0) && odd) {
 #pragma unroll
-        for (int j = 0; j < QB; ++j) {
-            top[j] = st[j][0][0];
+                for (int c = 0; c < 32; ++c)
+                    if (((0x000f000fu >> c) & 1) && ((odd >> c) & 1)) {
+                        const int node = key0 + c + fq * 4 - ctx;
+                        atomicOr(&s_odd[node >> 5 & 1], 1u << (node & 31));
+                    }
+            }
+            const int nb = key0 - ctx;                                   // node number of the tile's first key; negative: -nb context rows first
+            uint32_t there = 0;
 #pragma unroll
             for (int s = 0; s < SUB; ++s)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) top[j] = fmaxf(top[j], st[j][s][r]);
-            grow |= top[j] * a.scale_log2 > m[j] + 8.0f;                 // scale > 0: the maximum commutes with it
-        }
-        if (__any(grow)) {
+                if ((t.live >> s) & 1) there |= 0xffffu << (16 * s);
+            if (T_all - key0 < KT) there &= (1u << (T_all - key0)) - 1;
 #pragma unroll
             for (int j = 0; j < QB; ++j) {
-                float mx = fmaxf(top[j], __shfl_xor(top[j], 16, 64));
-                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                const float mn = mx * a.scale_log2 > m[j] + 8.0f ? mx * a.scale_log2 : m[j];      // by the query's own scores alone
-                const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[j] - mn);
-                l[j] *= alpha;
-                m[j] = mn;
-#pragma unroll
-                for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[j][dt][r] *= alpha;
+                const uint32_t w = nb >= 64 ? 0 : nb >= 0 ? (uint32_t)(see[j] >> nb) : nb <= -32 ? ~0u : ((uint32_t)see[j] << -nb) | ((1u << -nb) - 1);
+                win[j] = (w & there) >> (fq * 4);
             }
         }
+        if constexpr (QB == 4) tree_vt(t, vt);
+    };
+    // Query block by query block, so that the matrix unit works under the vector unit: the next block's scores and the last block's
+    // products run while one block's exponentials are taken.
+    auto use = [&](const Tile& t) {
+        f32x4 st[2][SUB];
+        tree_scores(kf, qf[0], st[0]);
 #pragma unroll
         for (int j = 0; j < QB; ++j) {
-            const float ms = m[j] == -INFINITY ? 0.f : m[j];             // nothing seen so far: keep the arguments finite
+            f32x4 (&p)[SUB] = st[j & 1];
+            if (edge) {
+#pragma unroll
+                for (int s = 0; s < SUB; ++s)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) p[s][r] = win[j] & (1u << (s * 16 + r)) ? p[s][r] : -INFINITY;
+            }
+            // The shift of the exponentials needs to be near the maximum, not the maximum: it follows only when a score lies more than
+            // 8 (a factor of 256 in a weight) above it, so that most tiles reduce nothing over lanes and scale nothing.
+            float top = p[0][0];
+#pragma unroll
+            for (int s = 0; s < SUB; ++s)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, p[s][r]);
+            if (__any(top > lim[j])) {                                   // scale > 0: the maximum commutes with it
+                float mx = fmaxf(top, __shfl_xor(top, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                if (mx > lim[j]) {                                       // by the query's own scores alone: its four lanes agree
+                    const float alpha = __builtin_amdgcn_exp2f(m[j] - mx * a.scale_log2);
+                    m[j] = mx * a.scale_log2;
+                    lim[j] = mx + 8.0f / a.scale_log2;
+                    shift[j] = -m[j];
+                    l[j] *= alpha;
+#pragma unroll
+                    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[j][dt][r] *= alpha;
+                }
+            }
+            if (j + 1 < QB) tree_scores(kf, qf[j + 1], st[(j + 1) & 1]);
             float sum = 0.f;
 #pragma unroll
             for (int s = 0; s < SUB; ++s)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(st[j][s][r], a.scale_log2, -ms));
-                    st[j][s][r] = p;
-                    sum += p;
+                    const float e = __builtin_amdgcn_exp2f(fmaf(p[s][r], a.scale_log2, shift[j]));
+                    p[s][r] = e;
+                    sum += e;
                 }
             l[j] += sum;
-        }
-        if (edge && __any(odd)) {
-            // A node's V row with infinities or NaN belongs to the queries that see it and to no other: 0 x inf in the MFMA
-            // would reach them all.  Such elements leave the tile and are added to the seeing queries alone, read once more.
-            uint32_t rows = 0;                                           // keys of the tile
-#pragma unroll
-            for (int s = 0; s < SUB; ++s)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const bool bad = key0 + s * 16 + fq * 4 + r >= ctx && tree_odd(t, s, r);
-                    const uint64_t lanes = __ballot(bad);
-#pragma unroll
-                    for (int f = 0; f < 4; ++f)
-                        if ((lanes >> (16 * f)) & 0xffff) rows |= 1u << (s * 16 + f * 4 + r);
-                    if (bad) tree_clean_v(t, s, r);
-                }
-            float* pl = &so[wave][0][0];                                 // the wave's own merge area: P as [key][16 queries]
-#pragma unroll
-            for (int j = 0; j < QB; ++j) {
-#pragma unroll
-                for (int s = 0; s < SUB; ++s)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) pl[(s * 16 + fq * 4 + r) * 16 + fr] = st[j][s][r];
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-                for (uint32_t left = rows; left; left &= left - 1) {
-                    const int kk = __builtin_ctz(left), key = key0 + kk;
-                    const float p = pl[kk * 16 + fr];
-                    const T* vp = vbase + tab[key >> a.shift] * page_stride + (long)(key & ((1 << a.shift) - 1)) * 64 + fq * 16;
-                    if (p > 0.f) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-#pragma unroll
-                            for (int dt = 0; dt < 4; ++dt) {
-                                const float v = to_f32<T>(vp[r * 4 + dt]);
-                                if (!(fabsf(v) < INFINITY)) o[j][dt][r] += p * v;
-                            }
-                    }
-                }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
+            if constexpr (QB != 4) {                                     // (the tile's registers are still its own: fewer live at once)
+                if (j == 0) tree_vt(t, vt);
             }
+            tree_pv(vt, p, o[j]);
         }
-        tree_pv<QB>(t, st, o);
     };
     if (mine > 0) {
-        Tile A, B;
-        int next = page_of(0);
-        load(A, 0, next);
-        next = page_of(1);
-        for (int i = 0;; i += 2) {
-            int after = page_of(i + 2);
-            load(B, i + 1, next);
-            __builtin_amdgcn_sched_barrier(0);                           // (left alone the compiler sinks the loads behind the products)
-            use(A, i);
-            if (i + 1 >= mine) break;
-            next = page_of(i + 3);
-            load(A, i + 2, after);
-            __builtin_amdgcn_sched_barrier(0);
-            use(B, i + 1);
-            if (i + 2 >= mine) break;
+        Tile A;
+        int after = page_of(0), next = page_of(1);                       // a page is requested one tile's loads ahead of its use
+        load(A, 0, after);
+        if constexpr (QB == 4) {                               // one set of registers: the next tile is requested once this one has left them
+            for (int i = 0; i < mine; ++i) {
+                after = page_of(i + 2);
+                open(A, i);
+                load(A, i + 1, next);
+                next = after;
+                __builtin_amdgcn_sched_barrier(0);                       // (left alone the compiler sinks the loads behind the products)
+                use(A);
+            }
+        } else {
+            Tile B;
+            for (int i = 0;; i += 2) {
+                after = page_of(i + 2);
+                load(B, i + 1, next);
+                __builtin_amdgcn_sched_barrier(0);
+                open(A, i);
+                use(A);
+                if (i + 1 >= mine) break;
+                next = page_of(i + 3);
+                load(A, i + 2, after);
+                __builtin_amdgcn_sched_barrier(0);
+                open(B, i + 1);
+                use(B);
+                if (i + 2 >= mine) break;
+            }
         }
     }
-    // ---- merge of the waves, one block of 16 queries at a time
-    constexpr int DPT = 16 / NW;                                         // dims per thread in the merge
-    const int mq = threadIdx.x / (64 / DPT), md = threadIdx.x % (64 / DPT) * DPT;
+    // ---- merge of the waves: a thread owns DPT dims of a query of every block
+    constexpr int DPT = 16 / NK;
+    typedef float part_t __attribute__((ext_vector_type(DPT)));
+    const int mg = threadIdx.x / (64 / DPT) / 16, mq = threadIdx.x / (64 / DPT) % 16, md = threadIdx.x % (64 / DPT) * DPT;
 #pragma unroll
     for (int j = 0; j < QB; ++j) {
-        if (q0 + j * 16 < nq) {                                          // uniform
         float lt = l[j];
         lt += __shfl_xor(lt, 16, 64);
         lt += __shfl_xor(lt, 32, 64);
-        if (j) __syncthreads();
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            *reinterpret_cast<f32x4*>(&so[wave][fr][(fq * 4 + r) * 4]) = f32x4{o[j][0][r], o[j][1][r], o[j][2][r], o[j][3][r]};
-        if (fq == 0) { sm[wave][fr] = m[j]; sl[wave][fr] = lt; }
-        __syncthreads();
-        const int qi = q0 + j * 16 + mq;
+            *reinterpret_cast<f32x4*>(&so[j][wave][fr][(fq * 4 + r) * 4]) = f32x4{o[j][0][r], o[j][1][r], o[j][2][r], o[j][3][r]};
+        if (fq == 0) { sm[j][wave][fr] = m[j]; sl[j][wave][fr] = lt; }
+    }
+    __syncthreads();
+    const uint64_t odd_nodes = ((uint64_t)s_odd[1] << 32) | s_odd[0];
+#pragma unroll
+    for (int j = 0; j < QB; ++j) {
+        const int qi = wg_q0 + mg * 16 * QB + j * 16 + mq;
         if (qi < nq) {
-            float M = -INFINITY, L = 0.f, acc[DPT] = {};
+            float M = -INFINITY, L = 0.f, mw[NK], lw[NK];
+            part_t acc = {}, ov[NK];
 #pragma unroll
-            for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w][mq]);
-#pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                const float sc = sm[w][mq] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[w][mq] - M);
-                if (sc == 0.f) continue;                                 // that wave saw nothing of weight
-                L += sl[w][mq] * sc;
-#pragma unroll
-                for (int d = 0; d < DPT; ++d) acc[d] += so[w][mq][md + d] * sc;
+            for (int k = 0; k < NK; ++k) {
+                const int w = k * NQ + mg;
+                mw[k] = sm[j][w][mq]; lw[k] = sl[j][w][mq];
+                ov[k] = *reinterpret_cast<const part_t*>(&so[j][w][mq][md]);
+                M = fmaxf(M, mw[k]);
             }
-            const int node = qi / a.g, head = kvh * a.g + qi % a.g;
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+                const float sc = mw[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw[k] - M);
+                L = sc == 0.f ? L : L + lw[k] * sc;                      // (a wave without weight leaves nothing, not 0 x infinity either)
+#pragma unroll
+                for (int d = 0; d < DPT; ++d) acc[d] = sc == 0.f ? acc[d] : acc[d] + ov[k][d] * sc;
+            }
+            const int node = node_of(qi), head = kvh * a.g + qi - node * a.g;
             const long row = r0 + node;
+            uint64_t odd = odd_nodes;
+            if (odd) {                                                   // infinities and NaN of the nodes this query sees
+                odd &= a.mask ? (uint64_t)a.mask[row] : (2ull << node) - 1;
+                for (; odd; odd &= odd - 1) {
+                    const int key = ctx + __builtin_ctzll(odd);
+                    const T* vp = vbase + tab[key >> a.shift] * page_stride + (long)(key & ((1 << a.shift) - 1)) * 64 + md;
+#pragma unroll
+                    for (int d = 0; d < DPT; ++d) {
+                        const float v = to_f32<T>(vp[d]);
+                        if (!(fabsf(v) < INFINITY)) acc[d] += v;
+                    }
+                }
+            }
             if (a.nsplit == 1) {
                 T* op = (T*)a.out + row * a.o_rs + head * 64 + md;
+                const float inv = L == 0.f ? 0.f : 1.0f / L;             // a row that sees nothing is zero
 #pragma unroll
-                for (int d = 0; d < DPT; ++d) op[d] = from_f32<T>(L == 0.f ? 0.f : acc[d] / L);     // a row that sees nothing is zero
+                for (int d = 0; d < DPT; ++d) op[d] = from_f32<T>(acc[d] * inv);
             } else {
                 const long at = (row * a.H + head) * a.nsplit + split;
-#pragma unroll
-                for (int d = 0; d < DPT; ++d) a.part[at * 64 + md + d] = acc[d];
+                *reinterpret_cast<part_t*>(a.part + at * 64 + md) = acc;
                 if (md == 0) {
                     float* ml = a.part + (long)a.rows * a.H * a.nsplit * 64 + at * 2;
                     ml[0] = M; ml[1] = L;
                 }
             }
         }
-        }
     }
 }
 
-// joins the workgroups' partial sums: one wave per (row, head), a lane per dimension
-template <typename T>
+// joins the workgroups' partial sums of a (row, head): one wave, a lane per dimension; or (many parts) four waves that deal them out
+template <typename T, int W>
 __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeArgs a) {
-    const int b = blockIdx.x, node = blockIdx.y, lane = threadIdx.x & 63;
-    const int head = blockIdx.z * 4 + (threadIdx.x >> 6);
+    const int b = blockIdx.x, node = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int head = W == 4 ? blockIdx.z : blockIdx.z * 4 + wave, first = W == 4 ? wave : 0;
     const int r0 = a.cu[b];
-    if (a.ctx[b] < 0 || r0 < 0 || head >= a.H) return;
+    if (a.ctx[b] < 0 || r0 < 0) return;
     if (node >= min(min(a.cu[b + 1] - r0, a.max_nodes), a.rows - r0)) return;
+    if (W == 1 && head >= a.H) return;
     const long row = r0 + node, at = (row * a.H + head) * a.nsplit;
     const float* ml = a.part + (long)a.rows * a.H * a.nsplit * 64 + at * 2;
     const float mv = lane < a.nsplit ? ml[2 * lane] : -INFINITY;
     const float lv = lane < a.nsplit ? ml[2 * lane + 1] : 0.f;
-    const float M = wave_max(mv);
-    const float w = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - M);
-    const float L = wave_sum(w == 0.f ? 0.f : lv * w);
-    float acc = 0.f;
-    for (int s0 = 0; s0 < a.nsplit; s0 += 8) {                           // eight loads under way
-        float v[8];
+    float acc = 0.f, M = 0.f, w = 0.f, L = 0.f;
+    for (int s0 = first; s0 < a.nsplit; s0 += 4 * W) {                   // four parts under way
+        float v[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = a.part[(at + min(s0 + i, a.nsplit - 1)) * 64 + lane];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float ws = s0 + i < a.nsplit ? __shfl(w, (s0 + i) & 63, 64) : 0.f;
-            acc = ws == 0.f ? acc : acc + v[i] * ws;                     // (a part that saw nothing wrote no sums)
+        for (int i = 0; i < 4; ++i) v[i] = a.part[(at + min(s0 + i * W, a.nsplit - 1)) * 64 + lane];
+        if (s0 == first) {
+            M = wave_max(mv);
+            w = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - M);
+            L = wave_sum(w == 0.f ? 0.f : lv * w);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = s0 + i * W;
+            const float ws = s < a.nsplit ? __shfl(w, s & 63, 64) : 0.f;
+            acc = ws == 0.f ? acc : acc + v[i] * ws;                     // (a part that saw nothing has no weight)
+        }
+    }
+    if constexpr (W == 4) {
+        __shared__ float red[4][64];
+        red[wave][lane] = acc;
+        __syncthreads();
+        if (wave) return;
+        acc = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
     }
     ((T*)a.out)[row * a.o_rs + head * 64 + lane] = from_f32<T>(L == 0.f ? 0.f : acc / L);
 }
 
-static int tree_qb(int nq) { return nq <= 16 ? 1 : nq <= 32 ? 2 : 4; }
+// The work of one (request, kv head): query blocks of 16 per wave (fp32 tiles leave registers for two) and query groups per workgroup.
+struct TreeShape { int qb, ng, blocks; };                               // blocks: workgroups over the queries
+static TreeShape tree_shape(int nq, int kt) {
+    TreeShape t;
+    t.qb = nq <= 16 ? 1 : nq <= 32 || kt == 16 ? 2 : 4;
+    const int groups = ceil_div(nq, 16 * t.qb);
+    t.ng = t.qb < 4 || groups == 1 ? 1 : groups == 2 ? 2 : 4;
+    t.blocks = ceil_div(groups, t.ng);
+    return t;
+}
 // Workgroups over the key axis: requests x kv heads x query blocks fill the chip alone from 256 on; below that the keys are
 // split until they do (two workgroups of one query block share a CU, larger ones have it alone), as long as a wave keeps two tiles.
 static int tree_splits(int B, int Hkv, int g, int max_nodes, int max_ctx, int kt, int nw) {
-    const int nq = max_nodes * g;
-    const long base = (long)B * Hkv * ceil_div(nq, 16 * tree_qb(nq));
+    const TreeShape t = tree_shape(max_nodes * g, kt);
+    const long base = (long)B * Hkv * t.blocks;
     const long tiles = ((long)max_ctx + max_nodes + kt - 1) / kt;
-    const long fill = tree_qb(nq) == 1 ? 512 : 256;
+    const long fill = t.qb == 1 ? 512 : 256;
     long s = (fill + base - 1) / base;
-    if (s > tiles / (2 * nw)) s = tiles / (2 * nw);
+    if (s > tiles / (2 * nw / t.ng)) s = tiles / (2 * nw / t.ng);
     if (base >= 256) s = 1;
     return (int)(s < 1 ? 1 : s > TREE_MAX_SPLIT ? TREE_MAX_SPLIT : s);
 }
 static bool tree_shape_ok(int rows, int B, int H, int Hkv, int max_nodes, int max_ctx) {
-    return rows >= 0 && B >= 0 && B <= 65535 && H > 0 && Hkv > 0 && H % Hkv == 0 && H <= 65535 && max_nodes > 0 && max_nodes <= TREE_MAX_NODES && max_ctx >= 0;
+    return rows >= 0 && B >= 0 && B <= 65535 && H > 0 && Hkv > 0 && H % Hkv == 0 && H <= 65535 && H / Hkv <= 1024 && max_nodes > 0 && max_nodes <= TREE_MAX_NODES && max_ctx >= 0;
 }
 #define TREE_NW 8
 
@@ -440,12 +498,17 @@ extern "C" size_t valle_attn_tree_workspace_bytes(int rows, int B, int max_nodes
 
 template <typename T>
 static void tree_launch(const TreeArgs& a, int B, hipStream_t s) {
-    const int nq = a.max_nodes * a.g, qb = tree_qb(nq);
-    dim3 grid(a.nsplit, a.Hkv * ceil_div(nq, 16 * qb), B);
-    if (qb == 1) attn_tree_kernel<T, 1, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
-    else if (qb == 2) attn_tree_kernel<T, 2, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
-    else attn_tree_kernel<T, 4, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
-    if (a.nsplit > 1) attn_tree_join_kernel<T><<<dim3(B, a.max_nodes, ceil_div(a.H, 4)), 256, 0, s>>>(a);
+    const TreeShape t = tree_shape(a.max_nodes * a.g, TreeTile<T>::SUB * 16);
+    const dim3 grid(a.nsplit, a.Hkv * t.blocks, B);
+    if (t.qb == 1) attn_tree_kernel<T, 1, 1, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
+    else if (t.qb == 2) attn_tree_kernel<T, 2, 1, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
+    else if constexpr (sizeof(T) == 2) {
+        if (t.ng == 1) attn_tree_kernel<T, 4, 1, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
+        else if (t.ng == 2) attn_tree_kernel<T, 4, 2, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
+        else attn_tree_kernel<T, 4, 4, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
+    }
+    if (a.nsplit > 16) attn_tree_join_kernel<T, 4><<<dim3(B, a.max_nodes, a.H), 256, 0, s>>>(a);
+    else if (a.nsplit > 1) attn_tree_join_kernel<T, 1><<<dim3(B, a.max_nodes, ceil_div(a.H, 4)), 256, 0, s>>>(a);
 }
 
 extern "C" int valle_attn_tree(const void* q, int64_t q_row_stride, const void* kcache, const void* vcache, int n_pages, int page_size,
@@ -463,6 +526,7 @@ extern "C" int valle_attn_tree(const void* q, int64_t q_row_stride, const void* 
     VALLE_REQUIRE(shift > 0, VALLE_E_ARG, "valle_attn_tree: page_size %d (16, 32, 64, 128 or 256)", page_size);
     VALLE_REQUIRE(n_pages > 0 && ((int64_t)n_pages << shift) <= INT32_MAX && max_blocks > 0 && ((int64_t)max_blocks << shift) <= INT32_MAX - (1 << 20), VALLE_E_ARG,
                   "valle_attn_tree: n_pages %d, max_blocks %d", n_pages, max_blocks);
+    VALLE_REQUIRE(((int64_t)Hkv << shift) * 64 * 4 <= INT32_MAX, VALLE_E_ARG, "valle_attn_tree: a page of %d kv heads is too large", Hkv);
     VALLE_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY, VALLE_E_ARG, "valle_attn_tree: softmax_scale must be positive");
     const int vec = 16 / (int)dtype_size(dtype);
     const void* ptrs[] = {q, kcache, vcache};
@@ -471,12 +535,12 @@ extern "C" int valle_attn_tree(const void* q, int64_t q_row_stride, const void* 
     VALLE_REQUIRE(rows <= 1 || out_row_stride >= (int64_t)H * 64, VALLE_E_ARG, "valle_attn_tree: rows of out overlap");
     if (B == 0 || rows == 0) return VALLE_OK;
     TreeArgs a{q, kcache, vcache, out, block_table, ctx_len, cu_rows, tree_mask, (float*)workspace, q_row_stride, out_row_stride,
-               softmax_scale * 1.4426950408889634f, max_blocks, n_pages, shift, rows, H, Hkv, H / Hkv, max_nodes, 1};
+               softmax_scale * 1.4426950408889634f, (uint32_t)(((1ull << 32) + H / Hkv - 1) / (H / Hkv)), max_blocks, n_pages, shift, rows, H, Hkv, H / Hkv, max_nodes, 1};
     a.nsplit = tree_splits(B, Hkv, a.g, max_nodes, max_ctx, dtype == VALLE_BF16 ? 32 : 16, TREE_NW);
     const size_t need = valle_attn_tree_workspace_bytes(rows, B, max_nodes, max_ctx, H, Hkv, dtype);
     VALLE_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), VALLE_E_WORKSPACE,
                   "valle_attn_tree: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
-    const long gy = (long)Hkv * ceil_div(max_nodes * a.g, 16 * tree_qb(max_nodes * a.g));
+    const long gy = (long)Hkv * tree_shape(max_nodes * (H / Hkv), dtype == VALLE_BF16 ? 32 : 16).blocks;
     VALLE_REQUIRE(gy <= 65535, VALLE_E_ARG, "valle_attn_tree: %d heads are too many", H);
     if (dtype == VALLE_BF16) tree_launch<bf16>(a, B, (hipStream_t)stream);
     else tree_launch<float>(a, B, (hipStream_t)stream);
