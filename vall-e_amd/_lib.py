@@ -18,6 +18,7 @@ EPI_GELU, EPI_RESID_BIAS = 6, 7
 
 _LIB_PATH = Path(__file__).resolve().parent / "libvalle_hip.so"
 _lib = None
+_serving = None
 
 c_void_p, c_int, c_float, c_size_t = C.c_void_p, C.c_int, C.c_float, C.c_size_t
 
@@ -169,6 +170,20 @@ def load():
     return lib
 
 
+def serving():
+    """The serving operators' native module (csrc/bind_serving.cpp).  Raises if it is absent."""
+    global _serving
+    if _serving is None:
+        load()
+        try:
+            from . import _serving as module
+        except ImportError as e:
+            raise ValleHipError(f"{_LIB_PATH.parent / '_serving.so'} is missing or does not load ({e}): build it first (python __graft_entry__.py)") from e
+        module.set_error(ValleHipError)
+        _serving = module
+    return _serving
+
+
 def check(rc: int):
     if rc != 0:
         msg = load().valle_last_error()
@@ -190,15 +205,6 @@ def ptr_any(t):
 
 def stream_ptr(device=None):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
-def raw_stream(index: int) -> int:
-    """Handle of the current stream of GPU ``index``.  ``torch.cuda.current_stream`` builds a Stream object around it (1.8 us per call on the
-    host, a third of a small operator's whole call)."""
-    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
-
-
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def dtype_code(dtype: torch.dtype) -> int:

@@ -171,41 +171,9 @@ class HipLinear4(torch.nn.Module):
         super()._load_from_state_dict(state_dict, prefix, *args, **kw)
 
     def forward(self, x, resid=None, geglu=False):
-        bufs, dev = self._buffers, x.get_device()          # (the dictionaries: a module's attribute lookup takes 0.4 us each)
-        wq, s, zeros, bias = bufs["wq"], bufs["scales"], bufs["zeros"], self._parameters["bias"]
-        if dev < 0:
-            raise L.ValleHipError("HipLinear4 needs GPU tensors; there is no CPU fallback")
-        if x.dtype is not s.dtype or s.get_device() != dev:
-            raise TypeError(f"HipLinear4: input {x.dtype} on {x.device}, scales {s.dtype} on {s.device}")
-        K, N, shape = self.in_features, self.out_features, x.shape
-        if shape[-1] != K:
-            raise ValueError(f"HipLinear4: input of width {shape[-1]}, {K} needed")
-        n_out, epi = N, L.EPI_STORE
-        if geglu:
-            if resid is not None or bias is not None or N % 2:
-                raise ValueError("HipLinear4: geglu takes an even number of columns, no bias and no residual")
-            n_out, epi = N // 2, L.EPI_GEGLU
-        x2 = x if len(shape) == 2 else x.reshape(-1, K)
-        rs, step = x2.stride()
-        if step != 1 or rs % 8 or rs > 1 << 23 or x2.data_ptr() % 16:
-            x2, rs = x2.clone(memory_format=torch.contiguous_format), K
-        out = x.new_empty((*shape[:-1], n_out))
-        if resid is not None:
-            if resid.shape != out.shape or resid.dtype is not x.dtype or resid.get_device() != dev:
-                raise ValueError(f"HipLinear4: residual {tuple(resid.shape)} {resid.dtype} for {tuple(out.shape)} {x.dtype}")
-            resid, epi = resid.contiguous(), L.EPI_RESID
-        if not len(x2):
-            return out
-        args = (x2.data_ptr(), rs, wq.data_ptr(), s.data_ptr(), None if zeros is None else zeros.data_ptr(), None if bias is None else bias.data_ptr(),
-                None if resid is None else resid.data_ptr(), out.data_ptr(), len(x2), N, K, self.group_size, n_out, epi, L.dtype_code(x.dtype))
-        if torch.cuda.current_device() == dev:
-            rc = L.load().valle_linear_w4(*args, L.raw_stream(dev))
-        else:
-            with torch.cuda.device(dev):
-                rc = L.load().valle_linear_w4(*args, L.raw_stream(dev))
-        if rc:
-            L.check(rc)
-        return out
+        b = self._buffers                                  # (the dictionary: a module's attribute lookup takes 0.4 us)
+        return L.serving().linear_w4(x, b["wq"], b["scales"], b["zeros"], self._parameters["bias"], resid, geglu, self.in_features, self.out_features,
+                                     self.group_size)
 
 
 class HipEmbedding(torch.nn.Module):
