@@ -72,8 +72,8 @@ __device__ __forceinline__ void plan_row(const PlanArgs& a, const int* ends, con
     a.slots[r] = plan_slot(a, b, p, stat[b] == 0);
     a.pos[r] = p;
 }
-// tree rows of one request: lane i = node i.  Ancestor bits and depths by pointer doubling (6 rounds cover 64 levels).
-__device__ __forceinline__ void plan_tree(const PlanArgs& a, int b, int start, int n, bool served, int lane) {
+// tree rows of one request: lane i = node i, its slot given.  Ancestor bits and depths by pointer doubling (6 rounds cover 64 levels).
+__device__ __forceinline__ void plan_tree(const PlanArgs& a, int len_old, int start, int n, int slot, int lane) {
     int up = -1;
     if (lane < n && start + lane < a.max_rows) {
         const int p = a.parents[start + lane];
@@ -85,14 +85,104 @@ __device__ __forceinline__ void plan_tree(const PlanArgs& a, int b, int start, i
     for (int it = 0; it < 6; ++it) {
         const int src = up >= 0 ? up : lane;
         const uint32_t lo = __shfl((uint32_t)m, src, 64), hi = __shfl((uint32_t)(m >> 32), src, 64);
-        const int d = __shfl(depth, src, 64), u = __shfl(up, src, 64);
-        if (up >= 0) { m |= ((uint64_t)hi << 32) | lo; depth += d; up = u; }
+        const int du = __shfl(depth << 8 | (up & 255), src, 64);         // depth and parent in one word: both stay below 64 (parent 255: none)
+        if (up >= 0) {
+            m |= ((uint64_t)hi << 32) | lo;
+            depth += du >> 8;
+            up = (du & 255) == 255 ? -1 : du & 255;
+        }
     }
     const int r = start + lane;
-    if (lane < n && r < a.max_rows) {
-        a.slots[r] = plan_slot(a, b, a.len_old[b] + lane, served);
-        a.pos[r] = a.len_old[b] + depth;
-        a.mask[r] = (int64_t)m;
+    if (lane < n && r < a.max_rows) { a.slots[r] = slot; a.pos[r] = len_old + depth; a.mask[r] = (int64_t)m; }
+}
+
+// inclusive sum over the lanes of a wave, on the cross-lane paths of the vector unit
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int plan_dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int plan_lane_scan(int v) {
+    v = plan_dpp_add<0x111, 0xf>(v);          // row_shr 1, 2, 4, 8: sums inside each row of 16
+    v = plan_dpp_add<0x112, 0xf>(v);
+    v = plan_dpp_add<0x114, 0xf>(v);
+    v = plan_dpp_add<0x118, 0xf>(v);
+    v = plan_dpp_add<0x142, 0xa>(v);          // row_bcast 15: the row before, into rows 1 and 3
+    return plan_dpp_add<0x143, 0xc>(v);       // row_bcast 31: rows 0 and 1, into rows 2 and 3
+}
+
+// Up to 64 requests: a request per lane, and every wave works the whole batch out for itself -- the sums cost a few dozen cycles, and what
+// the rows need is taken from the state as it was (a page that changes hands in this very call is looked up where it came from),
+// so the waves meet only once, between the reads of the counters and their writes (n_blocks_out may be n_blocks_in).  The latency is two
+// dependent memory round trips; the general form below takes five barriers.  16 requests with trees of 26 nodes: 7.3 -> 4.2 us.
+template <bool ROWS>
+__global__ __launch_bounds__(1024) void page_plan_small_kernel(PlanArgs a) {
+    __shared__ int s_f[64], s_from[64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool live = lane < a.B;
+    const int bl = live ? lane : 0;
+    const int lo = a.len_old[bl], ln = a.len_new[bl], held = a.nb_in[bl];
+    const int fc = min(max(*a.fc_in, 0), a.n_pages);
+    __syncthreads();
+    const long cap = (long)a.width << a.shift;
+    const bool valid = live && lo >= 0 && ln >= 0 && lo <= cap && ln <= cap && held >= 0 && held <= a.width && !(a.parents && ln - lo > 64);
+    const int want = valid ? (int)(((long)ln + (1 << a.shift) - 1) >> a.shift) : 0;
+    const int rows = valid && ln > lo ? ln - lo : 0;
+    const long end64 = (long)plan_lane_scan(rows & 0xffff) + ((long)plan_lane_scan(rows >> 16) << 16);
+    const int end = (int)min(end64, (long)INT32_MAX);
+    const bool ok = valid && end64 <= a.max_rows;
+    const int back = ok ? max(held - want, 0) : 0, need = ok ? max(want - held, 0) : 0;
+    const int f = plan_lane_scan(back), q = plan_lane_scan(need);
+    const int freed = __builtin_amdgcn_readlane(f, 63), F = fc + freed;
+    const bool served = ok && (need == 0 || q <= F);
+    const uint64_t takers = __ballot(served && need > 0);
+    const int taken = takers ? __shfl(q, 63 - __builtin_clzll(takers), 64) : 0;
+    if (wave == 0) {
+        if (live) {
+            a.cu[lane + 1] = end;
+            a.status[lane] = !valid ? 2 : !ok ? 3 : served ? 0 : 1;
+            a.nb_out[lane] = served ? want : held;
+        }
+        if (lane == 0) { a.cu[0] = 0; *a.fc_out = F - taken; }
+    }
+    s_f[lane] = f; s_from[lane] = want - (f - back);                     // (every wave writes the same)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    auto page_x = [&](int x) -> int {                                    // the page a request takes as number x: one given back in this call, or off the stack
+        if (x < freed) {
+            const int b = plan_find(s_f, a.B, x);
+            return a.table[(size_t)b * a.width + s_from[b] + x];
+        }
+        const int src = F - 1 - x;
+        return src >= 0 && src < a.n_pages ? a.free_list[src] : -1;
+    };
+    for (int b = wave; b < a.B; b += 16) {
+        const int lo_b = __builtin_amdgcn_readlane(lo, b), held_b = __builtin_amdgcn_readlane(held, b), want_b = __builtin_amdgcn_readlane(want, b);
+        const int back_b = __builtin_amdgcn_readlane(back, b), need_b = __builtin_amdgcn_readlane(need, b);
+        const int f0 = __builtin_amdgcn_readlane(f, b) - back_b, q0 = __builtin_amdgcn_readlane(q, b) - need_b;
+        const bool served_b = (__ballot(served) >> b) & 1;
+        int32_t* tab = a.table + (size_t)b * a.width;
+        for (int k = lane; k < back_b; k += 64) {
+            const int dst = F - 1 - (f0 + k);
+            if (dst >= 0 && dst < a.n_pages) a.free_list[dst] = tab[want_b + k];
+        }
+        if (served_b)
+            for (int k = lane; k < need_b; k += 64) tab[held_b + k] = page_x(q0 + k);
+        if constexpr (ROWS) {
+            const int end_b = __builtin_amdgcn_readlane(end, b), n = __builtin_amdgcn_readlane(rows, b), start = end_b - n;
+            auto slot_of = [&](int i) {                                  // of the request's new row i
+                const int p = lo_b + i, blk = p >> a.shift;
+                if (!served_b) return -1;
+                const int page = blk < held_b ? tab[blk] : page_x(q0 + blk - held_b);
+                return page >= 0 && page < a.n_pages ? (page << a.shift) + (p & ((1 << a.shift) - 1)) : -1;
+            };
+            if (a.parents) plan_tree(a, lo_b, start, n, lane < n ? slot_of(lane) : -1, lane);
+            else
+                for (int i = lane; i < n && start + i < a.max_rows; i += 64) { a.slots[start + i] = slot_of(i); a.pos[start + i] = lo_b + i; }
+        }
+    }
+    if constexpr (ROWS) {
+        for (int r = __builtin_amdgcn_readlane(end, 63) + threadIdx.x; r < a.max_rows; r += 1024) {
+            a.slots[r] = -1; a.pos[r] = 0;
+            if (a.parents) a.mask[r] = 0;
+        }
     }
 }
 
@@ -182,7 +272,7 @@ __global__ __launch_bounds__(NT) void page_plan_kernel(PlanArgs a) {
         if (a.parents) {
             for (int b = tid >> 6; b < a.B; b += NT / 64) {
                 const int start = b ? s_end[b - 1] : 0;
-                plan_tree(a, b, start, s_end[b] - start, s_f[b] == 0, tid & 63);
+                plan_tree(a, a.len_old[b], start, s_end[b] - start, (tid & 63) < s_end[b] - start ? plan_slot(a, b, a.len_old[b] + (tid & 63), s_f[b] == 0) : -1, tid & 63);
             }
             for (int r = s_end[a.B - 1] + tid; r < a.max_rows; r += NT) { a.slots[r] = -1; a.pos[r] = 0; a.mask[r] = 0; }
         } else {
@@ -198,7 +288,8 @@ __global__ __launch_bounds__(256) void page_rows_kernel(PlanArgs a) {
     if (a.parents) {
         for (int b = blockIdx.x * 4 + (threadIdx.x >> 6); b < a.B; b += gridDim.x * 4) {
             const int start = b ? s_end[b - 1] : 0;
-            plan_tree(a, b, start, s_end[b] - start, s_stat[b] == 0, threadIdx.x & 63);
+            const int i = threadIdx.x & 63, n = s_end[b] - start;
+            plan_tree(a, a.len_old[b], start, n, i < n ? plan_slot(a, b, a.len_old[b] + i, s_stat[b] == 0) : -1, i);
         }
         for (long r = (long)s_end[a.B - 1] + blockIdx.x * 256 + threadIdx.x; r < a.max_rows; r += gridDim.x * 256) {
             a.slots[r] = -1; a.pos[r] = 0; a.mask[r] = 0;
@@ -232,9 +323,11 @@ extern "C" int valle_page_plan(const int32_t* len_old, const int32_t* len_new, i
                parents, tree_mask, B, max_blocks, n_pages, shift, max_rows};
     hipStream_t s = (hipStream_t)stream;
     if (max_rows <= 4096) {
-        page_plan_kernel<1024, true><<<1, 1024, 0, s>>>(a);
+        if (B <= 64) page_plan_small_kernel<true><<<1, 1024, 0, s>>>(a);
+        else page_plan_kernel<1024, true><<<1, 1024, 0, s>>>(a);
     } else {
-        page_plan_kernel<1024, false><<<1, 1024, 0, s>>>(a);
+        if (B <= 64) page_plan_small_kernel<false><<<1, 1024, 0, s>>>(a);
+        else page_plan_kernel<1024, false><<<1, 1024, 0, s>>>(a);
         page_rows_kernel<<<min(ceil_div(max_rows, 256), 1024), 256, 0, s>>>(a);
     }
     VALLE_LAUNCH_CHECK();
