@@ -56,6 +56,11 @@ __device__ __forceinline__ void w4_store(const W4Args& a, int m, int n, const f3
     }
 }
 
+// Place (in 16 bytes) of piece c of row r in the wave's x: 8 consecutive lanes, the unit of a 16-byte LDS access, touch 8 different places
+// mod 8 whether they hold two rows x four pieces (the writes) or eight rows of one piece (the reads).  (With a rotation by 4 places per
+// piece the writes met in pairs: 9,200 of 39,000 cycles per CU at 8192 -> 8192, 40 rows.)
+__device__ __forceinline__ int w4_place(int r, int c) { return c * 16 + (((r & 7) | (((r >> 3) ^ (r >> 1)) & 1) << 3) ^ ((c & 3) << 1)); }
+
 // ---- the bf16 form.  A wave owns NT column tiles x MT row tiles and every NW-th k block; the loads of the next one are under way
 // while one is multiplied (two more under way: slower, 10.0 against 9.3 us at 8192 -> 8192).  Partial sums of the waves meet in LDS, in wave order.
 template <int GPB, int NT, int MT> struct W4Stage { uint4 w[NT]; uint2 s[GPB][NT]; uint32_t z[GPB][NT]; uint4 x[MT][4]; };
@@ -67,9 +72,9 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
     __shared__ f32x4 lds[NW * (NT > 4 ? NT : 4) * MT * 64];              // x of the waves, then their partial sums
     // x is loaded four lanes to a row (64 bytes in a piece; a row per lane, as the fragments have it, runs at a quarter of the rate)
-    // and turned to fragment order through the wave's own LDS; the rotation by 4 pieces per column keeps both sides free of conflicts.
+    // and turned to fragment order through the wave's own LDS.
     uint4* xl = reinterpret_cast<uint4*>(lds) + wave * MT * 4 * 64;
-    const int xw = (lane & 3) * 16 + (((lane >> 2) + 4 * (lane & 3)) & 15), xr = fq * 16 + ((fr + 4 * fq) & 15);
+    const int xw = w4_place(lane >> 2, lane & 3), xr = w4_place(fr, fq);
     const int rows = min(a.M - m0, 16 * MT);
     const __amdgpu_buffer_rsrc_t xb = buf_rsrc((const bf16*)a.x + (long)m0 * a.x_rs, (uint32_t)(((rows - 1) * a.x_rs + a.K) * 2));
     uint32_t xo[MT];
@@ -115,6 +120,9 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
             for (int t = 0; t < MT; ++t) xl[(j * MT + t) * 64 + xw] = st.x[t][j];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+        bf16x8 x[2][MT];                                                 // a fragment's rows, the next one's under way
+#pragma unroll
+        for (int t = 0; t < MT; ++t) x[0][t] = __builtin_bit_cast(bf16x8, xl[t * 64 + xr]);
 #pragma unroll
         for (int g = 0; g < GPB; ++g) {
             f32x4 xq[NT][MT], xs[MT];
@@ -127,19 +135,20 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
 #pragma unroll
             for (int f = 0; f < FPG; ++f) {
                 const int j = g * FPG + f;
-                if constexpr (MT == 3) __builtin_amdgcn_sched_barrier(0);
                 const bf16 one = (bf16)1.0f;
-                bf16x8 x[MT];
+                if (j < 3) {
 #pragma unroll
-                for (int t = 0; t < MT; ++t) x[t] = __builtin_bit_cast(bf16x8, xl[(j * MT + t) * 64 + xr]);
+                    for (int t = 0; t < MT; ++t) x[(j + 1) & 1][t] = __builtin_bit_cast(bf16x8, xl[((j + 1) * MT + t) * 64 + xr]);
+                }
+                if constexpr (MT == 3) __builtin_amdgcn_sched_barrier(0);        // (all four fragments' reads at once do not fit the registers)
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
-                    xs[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16x8{one, one, one, one, one, one, one, one}, x[t], xs[t], 0, 0, 0);
+                    xs[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16x8{one, one, one, one, one, one, one, one}, x[j & 1][t], xs[t], 0, 0, 0);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const bf16x8 q = w4_fragment(w4_word(st.w[n], j));
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) xq[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q, x[t], xq[n][t], 0, 0, 0);
+                    for (int t = 0; t < MT; ++t) xq[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q, x[j & 1][t], xq[n][t], 0, 0, 0);
                 }
             }
 #pragma unroll
@@ -156,15 +165,24 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     };
-    Stage st[2];
-    load(st[0], wave);
-    for (int kb = wave; kb < a.KB; kb += 2 * NW) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            if (kb + u * NW >= a.KB) break;
-            load(st[1 - u], kb + (u + 1) * NW);
+    if (a.KB <= NW) {                                                    // one block per wave: nothing to request ahead
+        Stage A;
+        if (wave < a.KB) {
+            load(A, wave);
+            use(A);
+        }
+    } else {
+        Stage A, B;
+        load(A, wave);
+        // (one way out, behind both halves' loads: from any other the compiler carries loads that are not under way into the loop's head
+        // and waits for those that are)
+        for (int kb = wave; kb < a.KB; kb += 2 * NW) {
+            load(B, kb + NW);
             __builtin_amdgcn_sched_barrier(0);                           // (left alone the compiler sinks the loads behind the products)
-            use(st[u]);
+            use(A);
+            load(A, kb + 2 * NW);
+            __builtin_amdgcn_sched_barrier(0);
+            if (kb + NW < a.KB) use(B);
         }
     }
     typedef f32x4 part_t[NT * MT][64];
@@ -229,11 +247,10 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_f32_kernel(W4Args a) {
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[0][t] = acc[1][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     auto use = [&](const Stage& st) {
-        // piece p (of 8) of row r at p * 16 + (r + 4 p) % 16: both sides free of bank conflicts
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int t = 0; t < MT; ++t) xl[((j >> 1) * MT + t) * 128 + ((j & 1) * 4 + pc) * 16 + ((rw + 4 * pc) & 15)] = st.x[t][j];
+            for (int t = 0; t < MT; ++t) xl[((j >> 1) * MT + t) * 128 + w4_place(rw, (j & 1) * 4 + pc)] = st.x[t][j];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -244,7 +261,7 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_f32_kernel(W4Args a) {
 #pragma unroll
             for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) x[t][e] = __builtin_bit_cast(f32x4, xl[(j * MT + t) * 128 + (2 * fq + e) * 16 + ((fr + 8 * fq + 4 * e) & 15)]);
+                for (int e = 0; e < 2; ++e) x[t][e] = __builtin_bit_cast(f32x4, xl[(j * MT + t) * 128 + w4_place(fr, 2 * fq + e)]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float w = (w4_value(w4_word(st.w, j), i) - z) * st.s[g];
@@ -255,15 +272,24 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_f32_kernel(W4Args a) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     };
-    Stage st[2];
-    load(st[0], wave);
-    for (int kb = wave; kb < a.KB; kb += 2 * NW) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            if (kb + u * NW >= a.KB) break;
-            load(st[1 - u], kb + (u + 1) * NW);
+    if (a.KB <= NW) {                                                    // one block per wave: nothing to request ahead
+        Stage A;
+        if (wave < a.KB) {
+            load(A, wave);
+            use(A);
+        }
+    } else {
+        Stage A, B;
+        load(A, wave);
+        // (one way out, behind both halves' loads: from any other the compiler carries loads that are not under way into the loop's head
+        // and waits for those that are)
+        for (int kb = wave; kb < a.KB; kb += 2 * NW) {
+            load(B, kb + NW);
+            __builtin_amdgcn_sched_barrier(0);                           // (left alone the compiler sinks the loads behind the products)
+            use(A);
+            load(A, kb + 2 * NW);
             __builtin_amdgcn_sched_barrier(0);
-            use(st[u]);
+            if (kb + NW < a.KB) use(B);
         }
     }
     typedef f32x4 part_t[MT][64];
