@@ -501,6 +501,35 @@ def test_attn_tree_siblings_with_infinities_and_nan(gpu_device, dtype, val):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ctx", [[30, 5], [3000, 2100]])
+def test_attn_tree_infinities_and_nan_that_are_seen_are_not_lost(gpu_device, dtype, ctx):
+    """NaN in a query reaches that row alone; NaN in a context key every row of its request and kv head, an infinity in a context value
+    every row's element of that dimension; nobody else's bits change.  (No key of a NaN query has a score with a maximum.)"""
+    args, mask, host = attn_case(gpu_device, dtype, ctx, [6, 18], 4, 2, 16, 12)
+    clean = P.attn_tree(*args, tree_mask=mask)
+    q, kc, vc, *rest = args
+    bad = q.clone()
+    bad[2, 1, 7] = float("nan")
+    got = P.attn_tree(bad, kc, vc, *rest, tree_mask=mask)
+    assert got[2, 1].isnan().all()
+    got[2, 1] = clean[2, 1]
+    assert torch.equal(got, clean)
+    for t in (0, 3, ctx[0] - 1):
+        at = (int(host[3][0, t // 16]), 0, t % 16)
+        bad = kc.clone()
+        bad[at] = float("nan")
+        got = P.attn_tree(q, bad, vc, *rest, tree_mask=mask)
+        assert got[:6, :2].isnan().all() and torch.equal(got[:6, 2:], clean[:6, 2:]) and torch.equal(got[6:], clean[6:])
+        bad = vc.clone()
+        bad[at][9] = float("inf")
+        got = P.attn_tree(q, kc, bad, *rest, tree_mask=mask)
+        assert not got[:6, :2, 9].isfinite().any()
+        got[:6, :2, 9] = clean[:6, :2, 9]
+        assert torch.equal(got, clean)
+
+
+@gpu
 def test_attn_tree_leaves_other_rows(gpu_device):
     """Rows behind the last request, of finished requests (negative ctx_len) and behind max_nodes stay as they were."""
     for ctx in ([50, 70, 40], [3000, 4000, 3500]):

@@ -387,9 +387,9 @@ __global__ __launch_bounds__(NW * 64, QB == 1 && sizeof(T) == 2 ? 4 : 2) void at
 #pragma unroll
             for (int k = 0; k < NK; ++k) {
                 const float sc = mw[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw[k] - M);
-                L = sc == 0.f ? L : L + lw[k] * sc;                      // (a wave without weight leaves nothing, not 0 x infinity either)
+                L += lw[k] * sc;                                         // (a wave whose scores are all NaN has no maximum, and its NaN goes on)
 #pragma unroll
-                for (int d = 0; d < DPT; ++d) acc[d] = sc == 0.f ? acc[d] : acc[d] + ov[k][d] * sc;
+                for (int d = 0; d < DPT; ++d) acc[d] += ov[k][d] * sc;
             }
             const int node = node_of(qi), head = kvh * a.g + qi - node * a.g;
             const long row = r0 + node;
@@ -444,13 +444,13 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeArgs a) {
         if (s0 == first) {
             M = wave_max(mv);
             w = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - M);
-            L = wave_sum(w == 0.f ? 0.f : lv * w);
+            L = wave_sum(lv * w);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int s = s0 + i * W;
-            const float ws = s < a.nsplit ? __shfl(w, s & 63, 64) : 0.f;
-            acc = ws == 0.f ? acc : acc + v[i] * ws;                     // (a part that saw nothing has no weight)
+            const float ws = __shfl(w, s & 63, 64);
+            if (s < a.nsplit) acc += v[i] * ws;                          // (a part that saw nothing holds zeros)
         }
     }
     if constexpr (W == 4) {

@@ -120,6 +120,7 @@ __global__ __launch_bounds__(1024) void page_plan_small_kernel(PlanArgs a) {
     const int bl = live ? lane : 0;
     const int lo = a.len_old[bl], ln = a.len_new[bl], held = a.nb_in[bl];
     const int fc = min(max(*a.fc_in, 0), a.n_pages);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                    // the counters are in registers before any of them is written over
     __syncthreads();
     const long cap = (long)a.width << a.shift;
     const bool valid = live && lo >= 0 && ln >= 0 && lo <= cap && ln <= cap && held >= 0 && held <= a.width && !(a.parents && ln - lo > 64);
