@@ -157,15 +157,17 @@ def test_linear_w4_shapes_views_and_rows_of_others(gpu_device):
 
 @gpu
 def test_linear_w4_rows_do_not_depend_on_their_neighbours(gpu_device):
-    """A row's result is the same bits alone, in a batch of 16 and in one of 64 (every output sums its k blocks in one order)."""
+    """A row's result is the same bits in a batch of 2, 16, 40 and 100, and in bf16 alone too (every output sums its k blocks in one order; a
+    single fp32 row takes a form of its own, with an order of its own)."""
     for dtype in (torch.bfloat16, torch.float32):
         q, s, z = make(64, 1024, 64, True, dtype, 2)
         d = lambda t: t.to(gpu_device)
         m = PL.HipLinear4.from_quantized(d(q), d(s), d(z))
         x = torch.randn(100, 1024, generator=torch.Generator().manual_seed(3)).to(dtype).to(gpu_device)
         full = m(x)
-        for rows in (1, 16, 40):
+        for rows in (1, 2, 16, 40) if dtype is torch.bfloat16 else (2, 16, 40):
             assert torch.equal(m(x[:rows]), full[:rows]), rows
+        check(m(x[:1]), *expect(x[:1].cpu(), q, s, z, 64), dtype)
 
 
 @gpu
@@ -184,3 +186,21 @@ def test_linear_w4_replaces_nn_linear(gpu_device):
     again = PL.HipLinear4(256, 96, bias=True, device=gpu_device, dtype=torch.float32)
     again.load_state_dict(m.state_dict())                                               # its own state dict, packed
     assert torch.equal(again(x), m(x))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,n,k,group", [(1, 1000, 4096, 64), (1, 72, 8320, 128), (1, 4100, 2336, 32), (1, 4112, 1216, 64), (40, 8200, 1408, 128), (33, 8192, 1216, 64),
+                                            (20, 8192, 1184, 32), (7, 8194, 3264, 64), (48, 4096, 4224, 128), (97, 200, 1184, 32)])
+def test_linear_w4_long_and_wide(gpu_device, dtype, rows, n, k, group):
+    """Several k blocks per wave in every form: last blocks that are no whole ones, an odd number of them, columns behind the last tile."""
+    q, s, z = make(n, k, group, True, dtype, n + k)
+    x = torch.randn(rows, k, generator=torch.Generator().manual_seed(k)).to(dtype)
+    d = lambda t: t.to(gpu_device)
+    m = PL.HipLinear4.from_quantized(d(q), d(s), d(z), group_size=group)
+    want = expect(x, q, s, z, group)
+    for _ in range(3):                                                                  # a race would differ
+        check(m(d(x)), *want, dtype)
+    pad = torch.full((rows, k + 8), float("nan"), dtype=dtype)
+    pad[:, :k] = x
+    check(m(d(pad)[:, :k]), *want, dtype)                                               # rows of a wider matrix: what lies between them is not theirs

@@ -94,6 +94,11 @@ __device__ __forceinline__ uint4 buf_load16(__amdgpu_buffer_rsrc_t r, uint32_t o
 __device__ __forceinline__ uint2 buf_load8(__amdgpu_buffer_rsrc_t r, uint32_t off) {
     return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
 }
+typedef __attribute__((address_space(3))) void buf_lds;
+// 16 bytes per lane from `off` to LDS, lane after lane behind the wave-uniform `to`
+__device__ __forceinline__ void buf_load16_lds(__amdgpu_buffer_rsrc_t r, char* to, uint32_t off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (buf_lds*)to, 16, off, 0, 0, 0);
+}
 __device__ __forceinline__ uint32_t buf_load4(__amdgpu_buffer_rsrc_t r, uint32_t off) { return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0); }
 
 static inline int ceil_div(int a, int b) { return (a + b - 1) / b; }

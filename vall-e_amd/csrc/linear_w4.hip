@@ -56,30 +56,42 @@ __device__ __forceinline__ void w4_store(const W4Args& a, int m, int n, const f3
     }
 }
 
-// Place (in 16 bytes) of piece c of row r in the wave's x: 8 consecutive lanes, the unit of a 16-byte LDS access, touch 8 different places
-// mod 8 whether they hold two rows x four pieces (the writes) or eight rows of one piece (the reads).  (With a rotation by 4 places per
-// piece the writes met in pairs: 9,200 of 39,000 cycles per CU at 8192 -> 8192, 40 rows.)
-__device__ __forceinline__ int w4_place(int r, int c) { return c * 16 + (((r & 7) | (((r >> 3) ^ (r >> 1)) & 1) << 3) ^ ((c & 3) << 1)); }
+// ---- the bf16 form.  A wave owns NT column tiles x MT row tiles and every NW-th k block.  x goes from L2 straight into the wave's own
+// LDS (no registers, no writes on the way), a ring of NS stages of two fragments (64 k): NS - 1 of them are always under way.  A
+// load is 16 rows x 64 bytes, four lanes to a row (a row per lane, as the fragments have it, runs at a quarter of the rate), and lands as it
+// comes, lane after lane; the 16-byte pieces of a row are asked for in the order c ^ (row / 2 mod 4), so that a fragment's read (eight
+// rows of one piece at a time) meets no bank twice.  Partial sums of the waves meet in LDS, in wave order.
+template <int GPB, int NT> struct W4Stage { uint4 w[NT]; uint2 s[GPB][NT]; uint32_t z[GPB][NT]; };
 
-// ---- the bf16 form.  A wave owns NT column tiles x MT row tiles and every NW-th k block; the loads of the next one are under way
-// while one is multiplied (two more under way: slower, 10.0 against 9.3 us at 8192 -> 8192).  Partial sums of the waves meet in LDS, in wave order.
-template <int GPB, int NT, int MT> struct W4Stage { uint4 w[NT]; uint2 s[GPB][NT]; uint32_t z[GPB][NT]; uint4 x[MT][4]; };
+// the two fragments of a stage, MT row tiles each (the compiler would wait for every load into LDS first)
+__device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[2][1]) {
+    asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:1024\n\ts_waitcnt lgkmcnt(0)" : "=&v"(x[0][0]), "=&v"(x[1][0]) : "v"(at) : "memory");
+}
+__device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[2][2]) {
+    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\tds_read_b128 %2, %4 offset:2048\n\tds_read_b128 %3, %4 offset:3072\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1]) : "v"(at) : "memory");
+}
+__device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[2][3]) {
+    asm volatile("ds_read_b128 %0, %6\n\tds_read_b128 %1, %6 offset:1024\n\tds_read_b128 %2, %6 offset:2048\n\tds_read_b128 %3, %6 offset:3072\n\t"
+                 "ds_read_b128 %4, %6 offset:4096\n\tds_read_b128 %5, %6 offset:5120\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[0][2]), "=&v"(x[1][0]), "=&v"(x[1][1]), "=&v"(x[1][2]) : "v"(at) : "memory");
+}
 
 template <int G, int NT, int MT, int NW>
 __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
     constexpr int GPB = 128 / G, FPG = G / 32;                           // groups per k block, fragments per group
+    constexpr int NS = MT == 3 ? 3 : 4, STAGE = 2 * MT * 1024;           // bytes of a stage
+    constexpr int AHEAD = (NS - 1) * 2 * MT + NT * (1 + 2 * GPB);        // loads that may be under way while a stage is multiplied: the next ones, the next weights
     const int nt0 = blockIdx.x * NT, m0 = blockIdx.y * 16 * MT, tiles = (a.N + 15) >> 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
-    __shared__ f32x4 lds[NW * (NT > 4 ? NT : 4) * MT * 64];              // x of the waves, then their partial sums
-    // x is loaded four lanes to a row (64 bytes in a piece; a row per lane, as the fragments have it, runs at a quarter of the rate)
-    // and turned to fragment order through the wave's own LDS.
-    uint4* xl = reinterpret_cast<uint4*>(lds) + wave * MT * 4 * 64;
-    const int xw = w4_place(lane >> 2, lane & 3), xr = w4_place(fr, fq);
-    const int rows = min(a.M - m0, 16 * MT);
+    __shared__ f32x4 lds[NW * NS * STAGE / 16];                          // x of the waves, then their partial sums
+    char* xl = reinterpret_cast<char*>(lds) + wave * NS * STAGE;
+    const uint32_t xr = (uint32_t)(uintptr_t)(buf_lds*)xl + fr * 64 + ((fq ^ (fr >> 1)) & 3) * 16;
+    const int rows = min(a.M - m0, 16 * MT), xrow = lane >> 2, xc = (lane ^ (xrow >> 1)) & 3;
     const __amdgpu_buffer_rsrc_t xb = buf_rsrc((const bf16*)a.x + (long)m0 * a.x_rs, (uint32_t)(((rows - 1) * a.x_rs + a.K) * 2));
     uint32_t xo[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) xo[t] = (uint32_t)(min(t * 16 + (lane >> 2), rows - 1) * a.x_rs + (lane & 3) * 8) * 2;   // rows behind the last: never stored
+    for (int t = 0; t < MT; ++t) xo[t] = (uint32_t)(min(t * 16 + xrow, rows - 1) * a.x_rs + xc * 8) * 2;   // rows behind the last: never stored
     __amdgpu_buffer_rsrc_t wb[NT], sb[NT], zb[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {                                       // tiles behind the last one read zeros
@@ -90,8 +102,8 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
         zb[n] = buf_rsrc(a.zeros + nt * a.KB * GPB * 16, on && a.zeros ? a.KB * GPB * 16 : 0);
     }
     const bool has_z = a.zeros != nullptr;
-    typedef W4Stage<GPB, NT, MT> Stage;
-    auto load = [&](Stage& st, int kb) {
+    typedef W4Stage<GPB, NT> Stage;
+    auto load_w = [&](Stage& st, int kb) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             st.w[n] = buf_load16(wb[n], kb * 1024 + lane * 16);
@@ -101,89 +113,92 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
                 st.z[g][n] = buf_load4(zb[n], (kb * GPB + g) * 16 + fq * 4);
             }
         }
+    };
+    // Stage i of this wave: half of block wave + NW (i / 2).  Behind the last block nothing moves; behind K (scales 0 there) the last
+    // fragment once more, which is a number wherever the row is.
+    auto load_x = [&](int i, int slot) {
+        const int kb = wave + NW * (i >> 1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int k = kb * 128 + j * 32;                             // K % 32 == 0: a fragment is in or out as a whole
+        for (int f = 0; f < 2; ++f) {
+            const int k = min(kb * 128 + (i & 1) * 64 + f * 32, a.K - 32);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) st.x[t][j] = buf_load16(xb, k < a.K ? xo[t] + k * 2 : BUF_OFF);
+            for (int t = 0; t < MT; ++t)
+                buf_load16_lds(xb, xl + slot * STAGE + (f * MT + t) * 1024, kb < a.KB ? xo[t] + k * 2 : BUF_OFF);
         }
     };
-    f32x4 acc[NT][MT];
+    f32x4 acc[NT][MT], xq[NT][MT], xs[MT];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int t = 0; t < MT; ++t) acc[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto use = [&](const Stage& st) {
+    auto use = [&](const Stage& st, int half, int slot) {
+        bf16x8 x[2][MT];
+        w4_read(xr + slot * STAGE, x);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int f = 0; f < 2; ++f) {
+            const int j = half * 2 + f, g = j / FPG;
+            const bf16 one = (bf16)1.0f;
+            const bf16x8 ones = bf16x8{one, one, one, one, one, one, one, one};
+            const f32x4 none = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int t = 0; t < MT; ++t) xl[(j * MT + t) * 64 + xw] = st.x[t][j];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        bf16x8 x[2][MT];                                                 // a fragment's rows, the next one's under way
-#pragma unroll
-        for (int t = 0; t < MT; ++t) x[0][t] = __builtin_bit_cast(bf16x8, xl[t * 64 + xr]);
-#pragma unroll
-        for (int g = 0; g < GPB; ++g) {
-            f32x4 xq[NT][MT], xs[MT];
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                xs[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int n = 0; n < NT; ++n) xq[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-            }
-#pragma unroll
-            for (int f = 0; f < FPG; ++f) {
-                const int j = g * FPG + f;
-                const bf16 one = (bf16)1.0f;
-                if (j < 3) {
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) x[(j + 1) & 1][t] = __builtin_bit_cast(bf16x8, xl[((j + 1) * MT + t) * 64 + xr]);
-                }
-                if constexpr (MT == 3) __builtin_amdgcn_sched_barrier(0);        // (all four fragments' reads at once do not fit the registers)
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
-                    xs[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16x8{one, one, one, one, one, one, one, one}, x[j & 1][t], xs[t], 0, 0, 0);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const bf16x8 q = w4_fragment(w4_word(st.w[n], j));
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) xq[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q, x[j & 1][t], xq[n][t], 0, 0, 0);
-                }
-            }
+            for (int t = 0; t < MT; ++t) xs[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, x[f][t], j % FPG ? xs[t] : none, 0, 0, 0);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const bf16x4 sv = __builtin_bit_cast(bf16x4, st.s[g][n]);
+                const bf16x8 q = w4_fragment(w4_word(st.w[n], j));
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float s = (float)sv[r], z = has_z ? (float)((st.z[g][n] >> (8 * r)) & 255u) : 8.0f;
+                for (int t = 0; t < MT; ++t) xq[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q, x[f][t], j % FPG ? xq[n][t] : none, 0, 0, 0);
+            }
+            if (j % FPG == FPG - 1) {
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) acc[n][t][r] = fmaf(s, fmaf(-z, xs[t][r], xq[n][t][r]), acc[n][t][r]);
+                for (int n = 0; n < NT; ++n) {
+                    const bf16x4 sv = __builtin_bit_cast(bf16x4, st.s[g][n]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float s = (float)sv[r], z = has_z ? (float)((st.z[g][n] >> (8 * r)) & 255u) : 8.0f;
+#pragma unroll
+                        for (int t = 0; t < MT; ++t) acc[n][t][r] = fmaf(s, fmaf(-z, xs[t][r], xq[n][t][r]), acc[n][t][r]);
+                    }
                 }
             }
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
     };
     if (a.KB <= NW) {                                                    // one block per wave: nothing to request ahead
         Stage A;
         if (wave < a.KB) {
-            load(A, wave);
-            use(A);
+            load_w(A, wave);
+            load_x(0, 0);
+            load_x(1, 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * MT) : "memory");
+            use(A, 0, 0);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            use(A, 1, 1);
         }
     } else {
         Stage A, B;
-        load(A, wave);
-        // (one way out, behind both halves' loads: from any other the compiler carries loads that are not under way into the loop's head
-        // and waits for those that are)
+        load_w(A, wave);
+#pragma unroll
+        for (int i = 0; i < NS - 1; ++i) load_x(i, i);
+        int slot = 0, i = 0;
+        auto step = [&](const Stage& st, int half, bool on) {            // asks for stage i + NS - 1, multiplies stage i
+            load_x(i + NS - 1, slot == 0 ? NS - 1 : slot - 1);
+            if (on) {
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(AHEAD) : "memory");
+                use(st, half, slot);
+            }
+            slot = slot == NS - 1 ? 0 : slot + 1;
+            ++i;
+        };
+        // (one way out, behind all loads: from any other the compiler carries loads that are not under way into the loop's head and
+        // waits for those that are)
         for (int kb = wave; kb < a.KB; kb += 2 * NW) {
-            load(B, kb + NW);
-            __builtin_amdgcn_sched_barrier(0);                           // (left alone the compiler sinks the loads behind the products)
-            use(A);
-            load(A, kb + 2 * NW);
-            __builtin_amdgcn_sched_barrier(0);
-            if (kb + NW < a.KB) use(B);
+            load_w(B, kb + NW);
+            step(A, 0, true);
+            step(A, 1, true);
+            load_w(A, kb + 2 * NW);
+            step(B, 0, kb + NW < a.KB);
+            step(B, 1, kb + NW < a.KB);
         }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                 // nothing more lands in LDS
     }
     typedef f32x4 part_t[NT * MT][64];
     part_t* part = reinterpret_cast<part_t*>(lds);
@@ -205,6 +220,11 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
         w4_store<bf16>(a, m0 + t * 16 + (l & 15), (nt0 + n) * 16 + (l >> 4) * 4, s);
     }
 }
+
+// Place (in 16 bytes) of piece c of row r in the wave's x: 8 consecutive lanes, the unit of a 16-byte LDS access, touch 8 different places
+// mod 8 whether they hold two rows x four pieces (the writes) or eight rows of one piece (the reads).  (With a rotation by 4 places per
+// piece the writes met in pairs: 9,200 of 39,000 cycles per CU at 8192 -> 8192, 40 rows.)
+__device__ __forceinline__ int w4_place(int r, int c) { return c * 16 + (((r & 7) | (((r >> 3) ^ (r >> 1)) & 1) << 3) ^ ((c & 3) << 1)); }
 
 // ---- the fp32 form: weights become (q - zero) * scale in fp32 (one rounding), the group structure ends there; an MFMA takes 4 inputs, the
 // k slots of a fragment are dealt so that a lane's 8 weights of a word meet its 8 values of x.  Two accumulators, for the dependent chain.
@@ -311,6 +331,84 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_f32_kernel(W4Args a) {
     }
 }
 
+// ---- fp32, one row: the vector unit's products (a matrix instruction would do 16 rows' work), and column tiles of CW = 4 so that a narrow
+// layer still fills the chip: lane = column, quarter of the 32 inputs of a word, and (CW = 4) one of four k blocks.  Sums whole numbers
+// times x per group, then scales: another order than the matrix form's, so a row alone is not bit-equal to the same row among others.
+template <int G, int CW, int NW>
+__global__ __launch_bounds__(NW * 64) void linear_w4_row_kernel(W4Args a) {
+    constexpr int GPB = 128 / G, BL = 16 / CW, FPG = G / 32;             // k blocks side by side in a wave
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane % CW, fq = lane / CW % 4, bl = lane / CW / 4;
+    const long nt = blockIdx.x / BL;
+    const int fr = blockIdx.x % BL * CW + c;                             // column in the tile of 16
+    const __amdgpu_buffer_rsrc_t xb = buf_rsrc(a.x, (uint32_t)a.K * 4);
+    const __amdgpu_buffer_rsrc_t wb = buf_rsrc(a.wq + nt * a.KB * 64, a.KB * 1024);
+    const __amdgpu_buffer_rsrc_t sb = buf_rsrc((const float*)a.scales + nt * a.KB * GPB * 16, a.KB * GPB * 64);
+    const __amdgpu_buffer_rsrc_t zb = buf_rsrc(a.zeros + nt * a.KB * GPB * 16, a.zeros ? a.KB * GPB * 16 : 0);
+    const bool has_z = a.zeros != nullptr;
+    struct Stage { uint4 w; uint32_t s[GPB], z[GPB]; uint4 x[8]; };
+    auto load = [&](Stage& st, int kb) {                                 // (behind the last block: zeros)
+        st.w = buf_load16(wb, kb * 1024 + (fq * 16 + fr) * 16);
+#pragma unroll
+        for (int g = 0; g < GPB; ++g) {
+            st.s[g] = buf_load4(sb, (kb * GPB + g) * 64 + fr * 4);
+            st.z[g] = buf_load4(zb, (kb * GPB + g) * 16 + (fr & 12));
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int k = kb * 128 + (j >> 1) * 32;
+            st.x[j] = buf_load16(xb, (uint32_t)(k + fq * 8 + (j & 1) * 4) * 4);
+        }
+    };
+    float acc = 0.f;
+    auto use = [&](const Stage& st) {
+        float p = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int g = j / FPG;
+            const float z = has_z ? (float)((st.z[g] >> ((fr & 3) * 8)) & 255u) : 8.0f;
+            if (j % FPG == 0) p = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float w = w4_value(w4_word(st.w, j), i) - z;       // exact
+                p = fmaf(w, __builtin_bit_cast(f32x4, st.x[2 * j + (i >> 2)])[i & 3], p);
+            }
+            if (j % FPG == FPG - 1) acc = fmaf(__builtin_bit_cast(float, st.s[g]), p, acc);
+        }
+    };
+    constexpr int STEP = NW * BL;
+    Stage A, B;
+    load(A, wave * BL + bl);
+    for (int kb = wave * BL; kb < a.KB; kb += 2 * STEP) {
+        load(B, kb + STEP + bl);
+        __builtin_amdgcn_sched_barrier(0);
+        use(A);
+        load(A, kb + 2 * STEP + bl);
+        __builtin_amdgcn_sched_barrier(0);
+        if (kb + STEP < a.KB) use(B);
+    }
+    __shared__ f32x4 part[NW][CW / 4];
+#pragma unroll
+    for (int o = CW; o < 64; o <<= 1) acc += __shfl_xor(acc, o, 64);
+    if (lane < CW) reinterpret_cast<float*>(&part[wave][0])[c] = acc;
+    __syncthreads();
+    if (threadIdx.x < CW / 4) {
+        const int i = threadIdx.x;
+        f32x4 v = part[0][i];
+#pragma unroll
+        for (int w = 1; w < NW; ++w)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += part[w][i][e];
+        w4_store<float>(a, 0, (int)nt * 16 + blockIdx.x % BL * CW + i * 4, v);
+    }
+}
+template <int G>
+static void w4_launch_row(const W4Args& a, hipStream_t s) {
+    const int tiles = ceil_div(a.N, 16);
+    if (tiles < 256) linear_w4_row_kernel<G, 4, 8><<<tiles * 4, 512, 0, s>>>(a);
+    else linear_w4_row_kernel<G, 16, 8><<<tiles, 512, 0, s>>>(a);
+}
+
 // Row tiles per workgroup: the fewest (more workgroups) that keep the launch within one workgroup per CU, else equal blocks of up to `most`.
 static int w4_row_tiles(int M, int gx, int most) {
     for (int mt = 1; mt < most; ++mt)
@@ -334,6 +432,9 @@ static void w4_launch(const W4Args& a, int dtype, hipStream_t s) {
         else w4_launch_bf16<G, 1>(a, s);
         return;
     }
+    // one row on the vector unit against the matrix form: 4096 -> 1024 4.1 / 9.8 us, 1024 -> 8192 5.7 / 5.8, 8192 -> 8192 12.5 / 27; two rows
+    // took 5.6 / 9.8, 9.1 / 5.8 and 23.8 / 27, four more than the matrix form everywhere
+    if (a.M == 1) return w4_launch_row<G>(a, s);
     // (two row tiles per workgroup take as long as two workgroups: 55.3 against 2 x 27.2 us at 8192 -> 8192; the MFMAs bound it)
     linear_w4_f32_kernel<G, 1, 8><<<dim3(ceil_div(a.N, 16), ceil_div(a.M, 16)), 512, 0, s>>>(a);
 }
