@@ -131,6 +131,26 @@ template <typename T> struct TreeVt;
 template <> struct TreeVt<bf16> { typedef bf16x8 type[4]; };
 template <> struct TreeVt<float> { typedef f32x4 type[4]; };
 
+// any infinity or NaN in the lane's part of a tile's V rows: exponent bits all ones carry into the sign's place
+__device__ __forceinline__ bool tree_any_odd(const TreeTile<bf16>& t) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint2 w = __builtin_bit_cast(uint2, t.v[s][r]);
+            any |= ((w.x & 0x7f807f80u) + 0x00800080u) | ((w.y & 0x7f807f80u) + 0x00800080u);
+        }
+    return (any & 0x80008000u) != 0;
+}
+__device__ __forceinline__ bool tree_any_odd(const TreeTile<float>& t) {
+    bool any = false;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any |= !(fabsf(t.v[0][r][e]) < INFINITY);
+    return any;
+}
 template <typename T>
 __device__ __forceinline__ bool tree_odd(const TreeTile<T>& t, int s, int r) {           // infinities or NaN in the lane's 4 dims of V row r
     bool odd = false;
@@ -145,21 +165,19 @@ __device__ __forceinline__ void tree_clean_v(TreeTile<T>& t, int s, int r) {
         if (!(fabsf(to_f32<T>(t.v[s][r][e])) < INFINITY)) t.v[s][r][e] = from_f32<T>(0.f);
 }
 
-// NQ groups of QB x 16 queries per workgroup: the waves of one key stream (there are NW / NQ) read the same tiles at about the same
-// time, so all but one of them find them in the CU's L1.
-template <typename T, int QB, int NQ, int NW>
+template <typename T, int QB, int NW>
 __global__ __launch_bounds__(NW * 64, QB == 1 && sizeof(T) == 2 ? 4 : 2) void attn_tree_kernel(TreeArgs a) {
     typedef TreeTile<T> Tile;
-    constexpr int SUB = Tile::SUB, KT = 16 * SUB, NK = NW / NQ;
+    constexpr int SUB = Tile::SUB, KT = 16 * SUB;
     const int split = blockIdx.x, kvh = blockIdx.y % a.Hkv, qblk = blockIdx.y / a.Hkv, b = blockIdx.z;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int fr = lane & 15, fq = lane >> 4, stream = wave / NQ;
+    const int fr = lane & 15, fq = lane >> 4;
     const int ctx_in = a.ctx[b], r0 = a.cu[b];
     if (ctx_in < 0 || r0 < 0) return;                                    // a finished request: its rows stay as they are
     const int nk = min(max(a.cu[b + 1] - r0, 0), TREE_MAX_NODES);        // nodes that are keys
     const int n = min(min(nk, a.max_nodes), a.rows - r0);                // nodes that ask
-    const int nq = n * a.g, wg_q0 = qblk * NQ * 16 * QB, q0 = wg_q0 + wave % NQ * 16 * QB;
-    if (n <= 0 || wg_q0 >= nq) return;
+    const int nq = n * a.g, q0 = qblk * 16 * QB;
+    if (n <= 0 || q0 >= nq) return;
     const int T_all = (int)min((long)ctx_in + nk, (long)a.width << a.shift);
     const int ctx = min(ctx_in, T_all);
     const int tiles = (T_all + KT - 1) / KT, per = (tiles + a.nsplit - 1) / a.nsplit;
@@ -195,10 +213,10 @@ __global__ __launch_bounds__(NW * 64, QB == 1 && sizeof(T) == 2 ? 4 : 2) void at
     __syncthreads();
     // Every load of the loop is issued whatever the case, through bounds-checked descriptors: what lies behind the wave's last tile
     // moves no data, and the loads stay countable.
-    const int mine = t0 + stream < t1 && q0 < nq ? (t1 - t0 - stream + NK - 1) / NK : 0;
+    const int mine = t0 + wave < t1 ? (t1 - t0 - wave + NW - 1) / NW : 0;
     const __amdgpu_buffer_rsrc_t tb = buf_rsrc(tab, a.width * 4);
     auto page_of = [&](int i) {                                          // lane s (mod SUB): the page of sub-tile s of this wave's tile i
-        const int key = (t0 + stream + NK * i) * KT + (lane % SUB) * 16;
+        const int key = (t0 + wave + NW * i) * KT + (lane % SUB) * 16;
         return (int)buf_load4(tb, i < mine && key < T_all ? (uint32_t)(key >> a.shift) * 4 : BUF_OFF);
     };
     auto load = [&](Tile& t, int i, int pages) {
@@ -207,7 +225,7 @@ __global__ __launch_bounds__(NW * 64, QB == 1 && sizeof(T) == 2 ? 4 : 2) void at
         asm("" : "+v"(ko), "+v"(vo));                                    // (kept next to the loads: their constants go into the instructions, not registers)
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
-            const int page = __builtin_amdgcn_readlane(pages, s), key = (t0 + stream + NK * i) * KT + s * 16;
+            const int page = __builtin_amdgcn_readlane(pages, s), key = (t0 + wave + NW * i) * KT + s * 16;
             const bool on = i < mine && key < T_all && page >= 0 && page < a.n_pages;
             const uint64_t at = (uint64_t)(uint32_t)(on ? page : 0) * page_bytes + (uint32_t)((key & ((1 << a.shift) - 1)) * 64 * (int)sizeof(T));
             const uint32_t bytes = on ? min(16, T_all - key) * 64 * (int)sizeof(T) : 0;      // rows behind the sequence read zeros
@@ -228,7 +246,7 @@ __global__ __launch_bounds__(NW * 64, QB == 1 && sizeof(T) == 2 ? 4 : 2) void at
     uint32_t win[QB];                                                    // bit s * 16 + r: the query sees key s * 16 + fq * 4 + r of the tile
     bool edge;
     auto open = [&](Tile& t, int i) {                                    // the tile leaves its registers: K over LDS into fragments, V turned
-        const int key0 = (t0 + stream + NK * i) * KT;
+        const int key0 = (t0 + wave + NW * i) * KT;
         uint4* kl = reinterpret_cast<uint4*>(&so[0][wave][0][0]);
         tree_stage_k(t, kl, lane);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -240,22 +258,24 @@ __global__ __launch_bounds__(NW * 64, QB == 1 && sizeof(T) == 2 ? 4 : 2) void at
         if (edge) {
             // A node's V row with infinities or NaN belongs to the queries that see it and to no other: 0 x inf in the MFMA would
             // reach them all.  Such elements are taken out here and added to the seeing queries in the merge.
-            uint32_t odd = 0;
+            if (__any(tree_any_odd(t))) {
+                uint32_t odd = 0;
 #pragma unroll
-            for (int s = 0; s < SUB; ++s)
+                for (int s = 0; s < SUB; ++s)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {                            // (rows behind the sequence were read as zeros)
-                    const bool bad = key0 + s * 16 + fq * 4 + r >= ctx && tree_odd(t, s, r);
-                    odd |= (uint32_t)bad << (s * 16 + r);
-                    if (bad) tree_clean_v(t, s, r);
-                }
-            if (__any(odd != 0) && odd) {
-#pragma unroll
-                for (int c = 0; c < 32; ++c)
-                    if (((0x000f000fu >> c) & 1) && ((odd >> c) & 1)) {
-                        const int node = key0 + c + fq * 4 - ctx;
-                        atomicOr(&s_odd[node >> 5 & 1], 1u << (node & 31));
+                    for (int r = 0; r < 4; ++r) {                            // (rows behind the sequence were read as zeros)
+                        const bool bad = key0 + s * 16 + fq * 4 + r >= ctx && tree_odd(t, s, r);
+                        odd |= (uint32_t)bad << (s * 16 + r);
+                        if (bad) tree_clean_v(t, s, r);
                     }
+                if (odd) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (((0x000f000fu >> c) & 1) && ((odd >> c) & 1)) {
+                            const int node = key0 + c + fq * 4 - ctx;
+                            atomicOr(&s_odd[node >> 5 & 1], 1u << (node & 31));
+                        }
+                }
             }
             const int nb = key0 - ctx;                                   // node number of the tile's first key; negative: -nb context rows first
             uint32_t there = 0;
@@ -356,9 +376,9 @@ __global__ __launch_bounds__(NW * 64, QB == 1 && sizeof(T) == 2 ? 4 : 2) void at
         }
     }
     // ---- merge of the waves: a thread owns DPT dims of a query of every block
-    constexpr int DPT = 16 / NK;
+    constexpr int DPT = 1024 / (NW * 64);
     typedef float part_t __attribute__((ext_vector_type(DPT)));
-    const int mg = threadIdx.x / (64 / DPT) / 16, mq = threadIdx.x / (64 / DPT) % 16, md = threadIdx.x % (64 / DPT) * DPT;
+    const int mq = threadIdx.x / (64 / DPT), md = threadIdx.x % (64 / DPT) * DPT;
 #pragma unroll
     for (int j = 0; j < QB; ++j) {
         float lt = l[j];
@@ -373,19 +393,18 @@ __global__ __launch_bounds__(NW * 64, QB == 1 && sizeof(T) == 2 ? 4 : 2) void at
     const uint64_t odd_nodes = ((uint64_t)s_odd[1] << 32) | s_odd[0];
 #pragma unroll
     for (int j = 0; j < QB; ++j) {
-        const int qi = wg_q0 + mg * 16 * QB + j * 16 + mq;
+        const int qi = q0 + j * 16 + mq;
         if (qi < nq) {
-            float M = -INFINITY, L = 0.f, mw[NK], lw[NK];
-            part_t acc = {}, ov[NK];
+            float M = -INFINITY, L = 0.f, mw[NW], lw[NW];
+            part_t acc = {}, ov[NW];
 #pragma unroll
-            for (int k = 0; k < NK; ++k) {
-                const int w = k * NQ + mg;
-                mw[k] = sm[j][w][mq]; lw[k] = sl[j][w][mq];
-                ov[k] = *reinterpret_cast<const part_t*>(&so[j][w][mq][md]);
+            for (int k = 0; k < NW; ++k) {
+                mw[k] = sm[j][k][mq]; lw[k] = sl[j][k][mq];
+                ov[k] = *reinterpret_cast<const part_t*>(&so[j][k][mq][md]);
                 M = fmaxf(M, mw[k]);
             }
 #pragma unroll
-            for (int k = 0; k < NK; ++k) {
+            for (int k = 0; k < NW; ++k) {
                 const float sc = mw[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw[k] - M);
                 L += lw[k] * sc;                                         // (a wave whose scores are all NaN has no maximum, and its NaN goes on)
 #pragma unroll
@@ -407,10 +426,12 @@ __global__ __launch_bounds__(NW * 64, QB == 1 && sizeof(T) == 2 ? 4 : 2) void at
                 }
             }
             if (a.nsplit == 1) {
-                T* op = (T*)a.out + row * a.o_rs + head * 64 + md;
+                typedef T out_t __attribute__((ext_vector_type(DPT)));
                 const float inv = L == 0.f ? 0.f : 1.0f / L;             // a row that sees nothing is zero
+                out_t y;
 #pragma unroll
-                for (int d = 0; d < DPT; ++d) op[d] = from_f32<T>(acc[d] * inv);
+                for (int d = 0; d < DPT; ++d) y[d] = from_f32<T>(acc[d] * inv);
+                *reinterpret_cast<out_t*>((T*)a.out + row * a.o_rs + head * 64 + md) = y;
             } else {
                 const long at = (row * a.H + head) * a.nsplit + split;
                 *reinterpret_cast<part_t*>(a.part + at * 64 + md) = acc;
@@ -463,27 +484,38 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeArgs a) {
     ((T*)a.out)[row * a.o_rs + head * 64 + lane] = from_f32<T>(L == 0.f ? 0.f : acc / L);
 }
 
-// The work of one (request, kv head): query blocks of 16 per wave (fp32 tiles leave registers for two) and query groups per workgroup.
-struct TreeShape { int qb, ng, blocks; };                               // blocks: workgroups over the queries
-static TreeShape tree_shape(int nq, int kt) {
-    TreeShape t;
-    t.qb = nq <= 16 ? 1 : nq <= 32 || kt == 16 ? 2 : 4;
-    const int groups = ceil_div(nq, 16 * t.qb);
-    t.ng = t.qb < 4 || groups == 1 ? 1 : groups == 2 ? 2 : 4;
-    t.blocks = ceil_div(groups, t.ng);
-    return t;
-}
-// Workgroups over the key axis: requests x kv heads x query blocks fill the chip alone from 256 on; below that the keys are
-// split until they do (two workgroups of one query block share a CU, larger ones have it alone), as long as a wave keeps two tiles.
-static int tree_splits(int B, int Hkv, int g, int max_nodes, int max_ctx, int kt, int nw) {
-    const TreeShape t = tree_shape(max_nodes * g, kt);
-    const long base = (long)B * Hkv * t.blocks;
+// How the work is cut: qb blocks of 16 queries per wave (fp32 tiles leave registers for two), `blocks` workgroups over the queries of a
+// (request, kv head), `split` over its keys.  A block more per wave saves key traffic and a wave's K and V turns, but costs registers (four
+// waves per SIMD at one block, two beyond), a longer start and end, and workgroups; splitting fills the chip but needs the join.  The
+// estimate in 0.1 us is fitted to measurements (bf16 unless said; us at 1 / 2 / 4 blocks; requests x context, nodes, heads / kv heads):
+//   1 x 130,001, 64, 16/4: 121 / 83 / 69     16 x 2,000, 64, 16/4: 35 / 29 / 23      16 x 536, 64, 16/4: 16.4 / 15.7 / 12.9
+//   32 x 2,200, 64, 16/16: 96 / 79 / 62      64 x 536, 26, 16/16: 33 / 40            16 x 536, 16, 16/4: 6.3 / 8.2 / 11.6
+//   1 x 64, 64, 16/4: 4.6 / 6.3 / 8.9        32 x 2,200, 26, 16/16: 57 / 52          fp32 1 x 300, 64, 16/16: 8.5 / 13.3; 16 x 64, 64, 16/16: 18.8 / 17.0
+struct TreeShape { int qb, blocks, split; };
+static TreeShape tree_shape(int B, int Hkv, int g, int max_nodes, int max_ctx, int kt) {
+    const int nq = max_nodes * g, nw = 8;
     const long tiles = ((long)max_ctx + max_nodes + kt - 1) / kt;
-    const long fill = t.qb == 1 ? 512 : 256;
-    long s = (fill + base - 1) / base;
-    if (s > tiles / (2 * nw / t.ng)) s = tiles / (2 * nw / t.ng);
-    if (base >= 256) s = 1;
-    return (int)(s < 1 ? 1 : s > TREE_MAX_SPLIT ? TREE_MAX_SPLIT : s);
+    TreeShape best{0, 0, 0};
+    double least = 0;
+    for (int qb = 1; qb <= (kt == 16 ? 2 : 4) && (qb == 1 || nq > 8 * qb); qb *= 2) {
+        const long blocks = ceil_div(nq, 16 * qb), base = (long)B * Hkv * blocks;
+        const long room = kt == 32 && qb == 1 ? 512 : 256;               // workgroups that run at a time
+        for (int whole = 1; whole >= 0; --whole) {
+            long split = whole ? 1 : room / base;
+            if (split > tiles / (2 * nw)) split = tiles / (2 * nw);      // (a wave keeps two tiles)
+            if (split > TREE_MAX_SPLIT) split = TREE_MAX_SPLIT;
+            if (split < 1 || (!whole && split == 1)) { if (!whole) continue; split = 1; }
+            const long groups = base * split, deep = (tiles + nw * split - 1) / (nw * split);
+            const double rounds = (double)((groups + room - 1) / room);
+            double t;
+            if (kt == 16) t = rounds * (qb == 1 ? 20 + 11.5 * deep : 40 + 22.0 * deep);
+            else if (qb == 1) t = groups <= 256 ? 8 + 8.0 * deep : rounds * (20 + 18.0 * deep);
+            else t = rounds * (qb == 2 ? 42 + 13.0 * deep : 50 + 18.0 * deep);
+            if (split > 1) t += 35 + (double)B * max_nodes * g * Hkv * split * 512 / 4e5;      // a launch, and the partial sums out and in at 4 TB/s
+            if (!best.qb || t < least) { best = TreeShape{qb, (int)blocks, (int)split}; least = t; }
+        }
+    }
+    return best;
 }
 static bool tree_shape_ok(int rows, int B, int H, int Hkv, int max_nodes, int max_ctx) {
     return rows >= 0 && B >= 0 && B <= 65535 && H > 0 && Hkv > 0 && H % Hkv == 0 && H <= 65535 && H / Hkv <= 1024 && max_nodes > 0 && max_nodes <= TREE_MAX_NODES && max_ctx >= 0;
@@ -492,21 +524,16 @@ static bool tree_shape_ok(int rows, int B, int H, int Hkv, int max_nodes, int ma
 
 extern "C" size_t valle_attn_tree_workspace_bytes(int rows, int B, int max_nodes, int max_ctx, int H, int Hkv, int dtype) {
     if (!tree_shape_ok(rows, B, H, Hkv, max_nodes, max_ctx) || B == 0) return 0;
-    const int ns = tree_splits(B, Hkv, H / Hkv, max_nodes, max_ctx, dtype == VALLE_BF16 ? 32 : 16, TREE_NW);
+    const int ns = tree_shape(B, Hkv, H / Hkv, max_nodes, max_ctx, dtype == VALLE_BF16 ? 32 : 16).split;
     return ns == 1 ? 0 : (size_t)rows * H * ns * 66 * sizeof(float);
 }
 
 template <typename T>
-static void tree_launch(const TreeArgs& a, int B, hipStream_t s) {
-    const TreeShape t = tree_shape(a.max_nodes * a.g, TreeTile<T>::SUB * 16);
+static void tree_launch(const TreeArgs& a, const TreeShape& t, int B, hipStream_t s) {
     const dim3 grid(a.nsplit, a.Hkv * t.blocks, B);
-    if (t.qb == 1) attn_tree_kernel<T, 1, 1, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
-    else if (t.qb == 2) attn_tree_kernel<T, 2, 1, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
-    else if constexpr (sizeof(T) == 2) {
-        if (t.ng == 1) attn_tree_kernel<T, 4, 1, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
-        else if (t.ng == 2) attn_tree_kernel<T, 4, 2, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
-        else attn_tree_kernel<T, 4, 4, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
-    }
+    if (t.qb == 1) attn_tree_kernel<T, 1, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
+    else if (t.qb == 2) attn_tree_kernel<T, 2, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
+    else if constexpr (sizeof(T) == 2) attn_tree_kernel<T, 4, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
     if (a.nsplit > 16) attn_tree_join_kernel<T, 4><<<dim3(B, a.max_nodes, a.H), 256, 0, s>>>(a);
     else if (a.nsplit > 1) attn_tree_join_kernel<T, 1><<<dim3(B, a.max_nodes, ceil_div(a.H, 4)), 256, 0, s>>>(a);
 }
@@ -529,21 +556,21 @@ extern "C" int valle_attn_tree(const void* q, int64_t q_row_stride, const void* 
     VALLE_REQUIRE(((int64_t)Hkv << shift) * 64 * 4 <= INT32_MAX, VALLE_E_ARG, "valle_attn_tree: a page of %d kv heads is too large", Hkv);
     VALLE_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY, VALLE_E_ARG, "valle_attn_tree: softmax_scale must be positive");
     const int vec = 16 / (int)dtype_size(dtype);
-    const void* ptrs[] = {q, kcache, vcache};
+    const void* ptrs[] = {q, kcache, vcache, out};
     for (const void* p : ptrs) VALLE_REQUIRE(((uintptr_t)p & 15) == 0, VALLE_E_ARG, "valle_attn_tree: tensors must be 16-byte aligned");
-    VALLE_REQUIRE(q_row_stride >= 0 && q_row_stride % vec == 0, VALLE_E_ARG, "valle_attn_tree: q rows must stay 16-byte aligned");
+    VALLE_REQUIRE(q_row_stride >= 0 && q_row_stride % vec == 0 && out_row_stride % vec == 0, VALLE_E_ARG, "valle_attn_tree: rows of q and out must stay 16-byte aligned");
     VALLE_REQUIRE(rows <= 1 || out_row_stride >= (int64_t)H * 64, VALLE_E_ARG, "valle_attn_tree: rows of out overlap");
     if (B == 0 || rows == 0) return VALLE_OK;
     TreeArgs a{q, kcache, vcache, out, block_table, ctx_len, cu_rows, tree_mask, (float*)workspace, q_row_stride, out_row_stride,
                softmax_scale * 1.4426950408889634f, (uint32_t)(((1ull << 32) + H / Hkv - 1) / (H / Hkv)), max_blocks, n_pages, shift, rows, H, Hkv, H / Hkv, max_nodes, 1};
-    a.nsplit = tree_splits(B, Hkv, a.g, max_nodes, max_ctx, dtype == VALLE_BF16 ? 32 : 16, TREE_NW);
+    const TreeShape shape = tree_shape(B, Hkv, a.g, max_nodes, max_ctx, dtype == VALLE_BF16 ? 32 : 16);
+    a.nsplit = shape.split;
     const size_t need = valle_attn_tree_workspace_bytes(rows, B, max_nodes, max_ctx, H, Hkv, dtype);
     VALLE_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), VALLE_E_WORKSPACE,
                   "valle_attn_tree: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
-    const long gy = (long)Hkv * tree_shape(max_nodes * (H / Hkv), dtype == VALLE_BF16 ? 32 : 16).blocks;
-    VALLE_REQUIRE(gy <= 65535, VALLE_E_ARG, "valle_attn_tree: %d heads are too many", H);
-    if (dtype == VALLE_BF16) tree_launch<bf16>(a, B, (hipStream_t)stream);
-    else tree_launch<float>(a, B, (hipStream_t)stream);
+    VALLE_REQUIRE((long)Hkv * shape.blocks <= 65535, VALLE_E_ARG, "valle_attn_tree: %d heads are too many", H);
+    if (dtype == VALLE_BF16) tree_launch<bf16>(a, shape, B, (hipStream_t)stream);
+    else tree_launch<float>(a, shape, B, (hipStream_t)stream);
     VALLE_LAUNCH_CHECK();
     return VALLE_OK;
 }
