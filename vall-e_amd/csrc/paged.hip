@@ -187,7 +187,7 @@ __global__ __launch_bounds__(1024) void page_plan_small_kernel(PlanArgs a) {
     }
 }
 
-// One workgroup plans the batch (a request per thread, up to four); ROWS: it also fills the rows, else page_rows_kernel does.
+// One workgroup plans the batch (a request per thread, up to four); ROWS: it also fills the rows (no trees), else page_rows_kernel does.
 template <int NT, bool ROWS>
 __global__ __launch_bounds__(NT) void page_plan_kernel(PlanArgs a) {
     constexpr int E = 4;
@@ -270,15 +270,7 @@ __global__ __launch_bounds__(NT) void page_plan_kernel(PlanArgs a) {
         for (int e = 0; e < E; ++e)
             if (e < per && b0 + e < a.B) s_f[b0 + e] = stat[e];
         __syncthreads();
-        if (a.parents) {
-            for (int b = tid >> 6; b < a.B; b += NT / 64) {
-                const int start = b ? s_end[b - 1] : 0;
-                plan_tree(a, a.len_old[b], start, s_end[b] - start, (tid & 63) < s_end[b] - start ? plan_slot(a, b, a.len_old[b] + (tid & 63), s_f[b] == 0) : -1, tid & 63);
-            }
-            for (int r = s_end[a.B - 1] + tid; r < a.max_rows; r += NT) { a.slots[r] = -1; a.pos[r] = 0; a.mask[r] = 0; }
-        } else {
-            for (int r = tid; r < a.max_rows; r += NT) plan_row(a, s_end, s_f, r);
-        }
+        for (int r = tid; r < a.max_rows; r += NT) plan_row(a, s_end, s_f, r);
     }
 }
 
@@ -323,13 +315,14 @@ extern "C" int valle_page_plan(const int32_t* len_old, const int32_t* len_new, i
     PlanArgs a{len_old, len_new, block_table, n_blocks_in, n_blocks_out, free_list, free_count_in, free_count_out, status, cu_rows, slots, positions,
                parents, tree_mask, B, max_blocks, n_pages, shift, max_rows};
     hipStream_t s = (hipStream_t)stream;
-    if (max_rows <= 4096) {
-        if (B <= 64) page_plan_small_kernel<true><<<1, 1024, 0, s>>>(a);
-        else page_plan_kernel<1024, true><<<1, 1024, 0, s>>>(a);
-    } else {
+    // The rows in the planning workgroup, or in a launch of their own over the chip: few rows of many requests 6.0 / 7.6 us (512 x 1), but
+    // trees beyond 64 requests 36.7 / 9.0 us (512 x 8), 13.4 / 8.3 (128 x 26): one wave per tree, sixteen at a time in one workgroup
+    if (max_rows <= 4096 && B <= 64) page_plan_small_kernel<true><<<1, 1024, 0, s>>>(a);
+    else if (max_rows <= 4096 && !parents) page_plan_kernel<1024, true><<<1, 1024, 0, s>>>(a);
+    else {
         if (B <= 64) page_plan_small_kernel<false><<<1, 1024, 0, s>>>(a);
         else page_plan_kernel<1024, false><<<1, 1024, 0, s>>>(a);
-        page_rows_kernel<<<min(ceil_div(max_rows, 256), 1024), 256, 0, s>>>(a);
+        page_rows_kernel<<<min(max(ceil_div(max_rows, 256), parents ? ceil_div(B, 4) : 0), 1024), 256, 0, s>>>(a);
     }
     VALLE_LAUNCH_CHECK();
     return VALLE_OK;
