@@ -3,7 +3,9 @@
 // 8-bit float (e4m3), exactly q * 2^-9 -- the subnormals and the first binade are one linear ramp -- so one conversion with a
 // scale of 512 makes two exact bf16 whole numbers.  The MFMA adds up x . q of one group in fp32, another one with an all-ones
 // fragment the sum of the group's x, and the accumulator takes scale * (x.q - zero * sum x) in fp32: no weight is ever rounded.
-// Bound: N K / 2 bytes of weights (plus scales and zeros) while the rows are few.
+// Bound: N K / 2 bytes of weights (plus scales and zeros) while the rows are few: 8192 -> 8192, group 128 (36 MB), 1 .. 16 rows 9.4 us
+// = 3.8 TB/s (8.2 without x's loads); a row tile of 16 more costs 4 us (32 rows 13.4, 40 rows 16.4): x passes through every CU whole,
+// 6 of the 16 us, and the row sums' products another 2.  Small layers are a launch and two round trips: 1024 -> 1024 2.9, 1024 -> 8192 3.5.
 //
 // Layout (the packer writes it once): k blocks of 128, columns in tiles of 16:
 //   wq   [N/16][K/128][64 lanes][16 bytes]: lane l = fq * 16 + fr holds column nt * 16 + fr; its word j (0 .. 3) the weights
@@ -57,7 +59,8 @@ __device__ __forceinline__ void w4_store(const W4Args& a, int m, int n, const f3
 }
 
 // ---- the bf16 form.  A wave owns NT column tiles x MT row tiles and every NW-th k block.  x goes from L2 straight into the wave's own
-// LDS (no registers, no writes on the way), a ring of NS stages of two fragments (64 k): NS - 1 of them are always under way.  A
+// LDS (no registers, no writes on the way; through registers 18.0 instead of 16.4 us at 8192 -> 8192, 40 rows), a ring of NS stages of two
+// fragments (64 k): NS - 1 of them are always under way, and the next block's weights (two blocks' weights: 16.8 us, and 9.9 for 9.4 at one row).  A
 // load is 16 rows x 64 bytes, four lanes to a row (a row per lane, as the fragments have it, runs at a quarter of the rate), and lands as it
 // comes, lane after lane; the 16-byte pieces of a row are asked for in the order c ^ (row / 2 mod 4), so that a fragment's read (eight
 // rows of one piece at a time) meets no bank twice.  Partial sums of the waves meet in LDS, in wave order.
@@ -162,7 +165,7 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
             }
         }
     };
-    if (a.KB <= NW) {                                                    // one block per wave: nothing to request ahead
+    if (a.KB <= NW) {                                                    // one block per wave: nothing to request ahead (1024 -> 8192: 3.5 against 4.0 us)
         Stage A;
         if (wave < a.KB) {
             load_w(A, wave);
@@ -409,7 +412,8 @@ static void w4_launch_row(const W4Args& a, hipStream_t s) {
     else linear_w4_row_kernel<G, 16, 8><<<tiles, 512, 0, s>>>(a);
 }
 
-// Row tiles per workgroup: the fewest (more workgroups) that keep the launch within one workgroup per CU, else equal blocks of up to `most`.
+// Row tiles per workgroup: the fewest (more workgroups) that keep the launch within one workgroup per CU, else equal blocks of up to `most`
+// (8192 -> 8192, 32 rows as one block of two 13.4 us, as two of one 2 x 9.4; 40 rows on 1024 -> 1024 as three of one 3.1).
 static int w4_row_tiles(int M, int gx, int most) {
     for (int mt = 1; mt < most; ++mt)
         if ((long)gx * ceil_div(M, 16 * mt) <= 256) return mt;
@@ -426,9 +430,9 @@ static void w4_launch_bf16(const W4Args& a, hipStream_t s) {
 template <int G>
 static void w4_launch(const W4Args& a, int dtype, hipStream_t s) {
     if (dtype == VALLE_BF16) {
-        // two column tiles per wave share the row fragments: from 256 workgroups of two tiles on, measured at 8192 -> 8192, group 128:
-        // 9.2 against 11.0 us for 1 .. 16 rows, 14.1 against 19.5 for 32; below, one (the chip would not be filled)
-        if (a.N >= 8192) w4_launch_bf16<G, 2>(a, s);
+        // Two column tiles per wave share the row fragments where that leaves a workgroup per CU; us with one / two: 8192 -> 8192, 1 row
+        // 10.8 / 9.5, 32 rows 19.9 / 13.4, 40 rows 24.2 / 16.1; 1024 -> 4096, 64 rows 5.7 / 4.3, but 16 rows (128 workgroups of two) 3.1 / 3.5.
+        if ((long)ceil_div(a.N, 32) * ceil_div(a.M, 48) >= 256) w4_launch_bf16<G, 2>(a, s);
         else w4_launch_bf16<G, 1>(a, s);
         return;
     }
