@@ -519,7 +519,9 @@ int valle_ar_decode_noalloc(valle_model* m, const valle_ar_state* st, const vall
  *                                served; -1 and position 0 behind the last row
  * With parents [max_rows] (tree_mask [max_rows] then too): row i of a request is a node whose parent is its row parents[.], an
  * earlier one (anything else: the context); its position is len_old + depth and tree_mask holds bit j for itself and every
- * ancestor j.  B <= 4096.  One launch up to 4,096 rows, two beyond. */
+ * ancestor j.  B <= 4096.  One launch up to 4,096 rows (with parents: and 64 requests), two beyond.  The lists must be whole: a page
+ * stands once in the stack or once in the first n_blocks entries of one request.  Rows of requests that are not served keep their
+ * numbers in cu_rows; what attention gives for them means nothing. */
 int valle_page_plan(const int32_t* len_old, const int32_t* len_new, int B, int page_size, int32_t* block_table, int max_blocks,
                     const int32_t* n_blocks_in, int32_t* n_blocks_out, int32_t* free_list, int n_pages,
                     const int32_t* free_count_in, int32_t* free_count_out, int32_t* status, int32_t* cu_rows,
@@ -528,7 +530,8 @@ int valle_page_plan(const int32_t* len_old, const int32_t* len_new, int B, int p
 /* valle_rope_kv for pages: q [M][H][64], k, v [M][Hkv][64] (row strides in elements, rows 16-byte aligned), q and k rotated by
  * rope[positions[m]] ([rope_rows][32][2] fp32; a position outside takes the nearest row), q to q_out (q_out == q is allowed; both
  * NULL: no q), k and v to slot slots[m] of the caches (a slot outside the pool: not written).  fp32 arithmetic, one rounding (in
- * bf16 valle_rope_kv rounds cos and sin first: not bit-equal).  Slots must differ from one another. */
+ * bf16 valle_rope_kv rounds cos and sin first: not bit-equal).  Slots must differ from one another (a slot named twice ends up
+ * with pieces of either row). */
 int valle_rope_kv_paged(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride,
                         void* q_out, int64_t q_out_row_stride, const int32_t* positions, const float* rope, int rope_rows,
                         const int32_t* slots, int M, int H, int Hkv, int Dh, void* kcache, void* vcache, int n_pages, int page_size,
@@ -538,8 +541,10 @@ int valle_rope_kv_paged(const void* q, int64_t q_row_stride, const void* k, int6
  * max_nodes <= 64 of them; rows behind that are left), cached at positions ctx_len[b] + i of its pages.  A row sees the ctx_len[b]
  * context rows and the nodes whose bit is set in its tree_mask (NULL: rows 0 .. itself); H % Hkv == 0, head h reads kv head
  * h / (H / Hkv).  A row that sees nothing gives zeros; requests with ctx_len < 0 and rows of no request are left as they were.
- * Rows of a page behind the sequence, and nodes a row does not see, may hold anything (infinities, NaN).  max_ctx: host-side
- * estimate of the longest context; it only chooses how the keys are split.  workspace: valle_attn_tree_workspace_bytes with the
+ * Rows of a page behind the sequence, and nodes a row does not see, may hold anything (infinities, NaN); what a row does see goes
+ * into its sums as it is.  Positions at and behind max_blocks * page_size are not there.  H / Hkv <= 1024, max_blocks * page_size <= 2^31 - 2^20, q and out
+ * 16-byte aligned row by row; out may be q.  A row's result does not depend on what the other rows hold.  max_ctx: host-side estimate of the longest
+ * context; it only chooses how the keys are split (and with it the order of the sums).  workspace: valle_attn_tree_workspace_bytes with the
  * same numbers (0: none needed), 16-byte aligned, not shared by calls that may overlap. */
 size_t valle_attn_tree_workspace_bytes(int rows, int B, int max_nodes, int max_ctx, int H, int Hkv, int dtype);
 int valle_attn_tree(const void* q, int64_t q_row_stride, const void* kcache, const void* vcache, int n_pages, int page_size,
@@ -549,7 +554,8 @@ int valle_attn_tree(const void* q, int64_t q_row_stride, const void* kcache, con
 
 /* The accepted path of every tree becomes context, in all layers (layer_stride elements apart): cached row ctx_len[b] + path[b][j]
  * moves to ctx_len[b] + j, j < min(n_accept[b], max_path), max_path <= 64; a node number outside 0 .. 63 moves nothing.  All of a
- * request's rows are read before any is written.  len_out[b] = ctx_len[b] + n_accept[b] (not ctx_len itself; negative lengths stay). */
+ * request's rows are read before any is written.  len_out[b] = ctx_len[b] + n_accept[b] (not ctx_len itself; negative lengths stay).
+ * n_accept must not pass the rows that were planned: pages behind n_blocks belong to others. */
 int valle_paged_kv_commit(void* kcache, void* vcache, int n_layers, int64_t layer_stride, const int32_t* block_table, int max_blocks,
                           int n_pages, int page_size, const int32_t* ctx_len, const int32_t* path, int max_path,
                           const int32_t* n_accept, int32_t* len_out, int B, int Hkv, int Dh, int dtype, void* stream);
@@ -560,7 +566,9 @@ int valle_paged_kv_commit(void* kcache, void* vcache, int n_layers, int64_t laye
  *   wq [N/16][K/128][64][16 bytes]  lane l = fq * 16 + fr: column fr of the tile; word j, byte i: inputs j * 32 + fq * 8 + i (low nibble) and
  *                                   + i + 4 (high nibble)
  *   scales [N/16][(K/128) * (128/group)][16] in dtype, zeros the same in bytes (NULL: 8)
- * x: row stride in elements, rows 16-byte aligned.  Epilogues STORE (+ bias), RESID (+ bias, + resid [M][ldc]), GEGLU (no bias), F32OUT. */
+ * x: row stride in elements (0 .. 2^23), rows 16-byte aligned.  A row of x with infinities or NaN gives such, its row alone; values whose sums
+ * of 15 |x| over a group pass the fp32 range overflow.  A row's result does not depend on its neighbours, but a single fp32 row is summed in
+ * another order than one of several.  Epilogues STORE (+ bias), RESID (+ bias, + resid [M][ldc]), GEGLU (no bias), F32OUT. */
 int valle_linear_w4(const void* x, int64_t x_row_stride, const void* wq, const void* scales, const uint8_t* zeros, const void* bias,
                     const void* resid, void* C, int M, int N, int K, int group, int ldc, int epilogue, int dtype, void* stream);
 

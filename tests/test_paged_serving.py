@@ -567,6 +567,39 @@ def test_attn_tree_views_scale_and_streams(gpu_device):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ctx,nodes,H,kv", [([40, 90], [30, 8], 8, 2), ([2500], [40], 4, 1), ([9, 0, 70], [1, 1, 1], 3, 3)])
+def test_attn_tree_result_in_place_of_the_queries(gpu_device, dtype, ctx, nodes, H, kv):
+    """out=q, with several query blocks and with split keys: the same bits as into a tensor of its own."""
+    args, mask, host = attn_case(gpu_device, dtype, ctx, nodes, H, kv, 16, 14)
+    want = P.attn_tree(*args, tree_mask=mask, max_nodes=max(nodes), max_ctx=max(ctx))
+    q = args[0].clone()
+    assert P.attn_tree(q, *args[1:], tree_mask=mask, max_nodes=max(nodes), max_ctx=max(ctx), out=q) is q and torch.equal(q, want)
+
+
+@gpu
+def test_attn_tree_more_heads_than_a_grid_of_small_blocks_holds(gpu_device):
+    """20,480 heads in groups of 1,024, 64 nodes: query blocks are taken as large as the grid needs; too many are refused."""
+    from vall_e_amd import _lib as L
+    kc, vc = randn((2, 20, 16, 64), torch.bfloat16, 1, gpu_device), randn((2, 20, 16, 64), torch.bfloat16, 2, gpu_device)
+    q = randn((64, 20 * 1024, 64), torch.bfloat16, 3, gpu_device)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=gpu_device)
+    got = P.attn_tree(q, kc, vc, i32([[1, 0, 0, 0, 0]]), i32([16]), i32([0, 64]))
+    rows, heads = [0, 1, 5], [0, 1023, 1024, 20479]                                      # a chain: row i sees itself and what lies before it
+    for r in rows:
+        for h in heads:
+            k = torch.cat((kc[1, h // 1024], kc[0, h // 1024]))[:17 + r].double().cpu()
+            v = torch.cat((vc[1, h // 1024], vc[0, h // 1024]))[:17 + r].double().cpu()
+            w = torch.softmax(k @ q[r, h].double().cpu() * 0.125, 0)
+            ds = 70 * U32 * 0.125 * float((k.abs() @ q[r, h].double().cpu().abs()).max())
+            lim = (2.2 * ds + 81 * U32 + 2.0 ** -8) * (w @ v.abs()) + 2.0 ** -8 * (w @ v).abs()
+            assert ((got[r, h].cpu().double() - w @ v).abs() <= lim).all()
+    kc, vc = (torch.zeros(2, 63, 16, 64, device=gpu_device) for _ in range(2))
+    with pytest.raises(L.ValleHipError, match="too many"):
+        P.attn_tree(torch.zeros(64, 63 * 1024, 64, device=gpu_device), kc, vc, i32([[1, 0]]), i32([16]), i32([0, 64]))
+
+
+@gpu
 def test_attn_tree_one_token_equals_the_slot_cache_operator(gpu_device):
     """One node per request over pages == valle_attn_decode over slots, both within the bound of the fp64 result."""
     from vall_e_amd import _lib as L

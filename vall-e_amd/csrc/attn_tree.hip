@@ -504,6 +504,7 @@ static TreeShape tree_shape(int B, int Hkv, int g, int max_nodes, int max_ctx, i
     double least = 0;
     for (int qb = 1; qb <= (kt == 16 ? 2 : 4) && (qb == 1 || nq > 8 * qb); qb *= 2) {
         const long blocks = ceil_div(nq, 16 * qb), base = (long)B * Hkv * blocks;
+        if (Hkv * blocks > 65535) continue;                              // (no such grid)
         const long room = kt == 32 && qb == 1 ? 512 : 256;               // workgroups that run at a time
         for (int whole = 1; whole >= 0; --whole) {
             long split = whole ? 1 : room / base;
@@ -530,7 +531,7 @@ static bool tree_shape_ok(int rows, int B, int H, int Hkv, int max_nodes, int ma
 extern "C" size_t valle_attn_tree_workspace_bytes(int rows, int B, int max_nodes, int max_ctx, int H, int Hkv, int dtype) {
     if (!tree_shape_ok(rows, B, H, Hkv, max_nodes, max_ctx) || B == 0) return 0;
     const int ns = tree_shape(B, Hkv, H / Hkv, max_nodes, max_ctx, dtype == VALLE_BF16 ? 32 : 16).split;
-    return ns == 1 ? 0 : (size_t)rows * H * ns * 66 * sizeof(float);
+    return ns <= 1 ? 0 : (size_t)rows * H * ns * 66 * sizeof(float);
 }
 
 template <typename T>
@@ -573,7 +574,7 @@ extern "C" int valle_attn_tree(const void* q, int64_t q_row_stride, const void* 
     const size_t need = valle_attn_tree_workspace_bytes(rows, B, max_nodes, max_ctx, H, Hkv, dtype);
     VALLE_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), VALLE_E_WORKSPACE,
                   "valle_attn_tree: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
-    VALLE_REQUIRE((long)Hkv * shape.blocks <= 65535, VALLE_E_ARG, "valle_attn_tree: %d heads are too many", H);
+    VALLE_REQUIRE(shape.qb, VALLE_E_ARG, "valle_attn_tree: %d heads are too many", H);
     if (dtype == VALLE_BF16) tree_launch<bf16>(a, shape, B, (hipStream_t)stream);
     else tree_launch<float>(a, shape, B, (hipStream_t)stream);
     VALLE_LAUNCH_CHECK();

@@ -407,7 +407,7 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_row_kernel(W4Args a) {
 }
 template <int G>
 static void w4_launch_row(const W4Args& a, hipStream_t s) {
-    const int tiles = ceil_div(a.N, 16);
+    const int tiles = ceil_div(a.N, 16);                                 // us with CW = 4 / 16: 4096 -> 1024 4.2 / 5.4, 1024 -> 2048 3.4 / 3.9; 1024 -> 4096 5.0 / 4.0
     if (tiles < 256) linear_w4_row_kernel<G, 4, 8><<<tiles * 4, 512, 0, s>>>(a);
     else linear_w4_row_kernel<G, 16, 8><<<tiles, 512, 0, s>>>(a);
 }

@@ -49,7 +49,7 @@ class PageTable:
     Written by every ``plan``: ``cu_rows`` [max_requests + 1] (row offsets of the step's packed rows), ``slots`` / ``positions``
     [max_rows] (slot = page * page_size + offset; -1: padding row, or a request without pages), ``tree_mask`` [max_rows] int64
     (with ``parents`` only), ``status`` [max_requests]: 0 served, 1 no pages left (it keeps what it had), 2 lengths out of range,
-    3 its rows lie behind ``max_rows``."""
+    3 its rows lie behind ``max_rows``; what a step computes for rows of requests that were not served means nothing."""
 
     def __init__(self, max_requests, max_blocks, n_pages, page_size, max_rows, device="cuda"):
         _need(page_size in PAGE_SIZES, f"page_size {page_size}: one of {PAGE_SIZES}")
@@ -89,7 +89,7 @@ class PageTable:
 def rope_kv_paged(q, k, v, positions, rope, slots, k_cache, v_cache, out=None):
     """RoPE on the rows' q and k (``[rows][heads][64]``, views of a fused projection work as they are), k and v written into the
     pages: row r goes to slot ``slots[r]`` of ``k_cache`` / ``v_cache`` ``[n_pages][kv_heads][page_size][64]`` (a slot outside the
-    pool, -1 for instance: not written; a slot named twice: either row).  ``rope`` fp32 ``[positions][32][2]`` = (cos, sin);
+    pool, -1 for instance: not written; a slot named twice: pieces of either row).  ``rope`` fp32 ``[positions][32][2]`` = (cos, sin);
     positions outside the table take its nearest row.  Returns the rotated q (``out``, which may be q itself)."""
     return _S.rope_kv_paged(q, k, v, positions, rope, slots, k_cache, v_cache, out)
 
@@ -99,7 +99,7 @@ def attn_tree(q, k_cache, v_cache, block_table, ctx_len, cu_rows, tree_mask=None
     (``[rows][heads][64]``, heads a multiple of the cache's kv_heads; up to 64 rows per request), which see all of its
     ``ctx_len[b]`` cached rows and, of the new rows (cached behind them), those whose bit is set in ``tree_mask[row]`` (None: a
     chain, row i sees rows 0 .. i; one row: a plain decode step).  A row that sees nothing is zero.  Requests with a negative
-    ``ctx_len`` and rows behind ``cu_rows[-1]`` are left as they were (``out=`` to say what that is).  ``max_nodes``: the largest
+    ``ctx_len`` and rows behind ``cu_rows[-1]`` are left as they were (``out=`` to say what that is; it may be q).  ``max_nodes``: the largest
     number of rows of a request (default: as many as can be; rows behind it are left), ``max_ctx``: the longest context, a hint
     for how to split the work."""
     return _S.attn_tree(q, k_cache, v_cache, block_table, ctx_len, cu_rows, tree_mask, max_nodes, max_ctx,
@@ -109,6 +109,6 @@ def attn_tree(q, k_cache, v_cache, block_table, ctx_len, cu_rows, tree_mask=None
 def kv_commit(k_cache, v_cache, block_table, ctx_len, path, n_accept):
     """The accepted nodes of every request's tree become context, in all layers: cached row ``ctx_len[b] + path[b][j]`` moves to
     ``ctx_len[b] + j`` for ``j < n_accept[b]`` (``path`` int32 [requests][up to 64], node numbers 0 .. 63; others stay where they
-    are).  Caches ``[n_layers][n_pages][kv_heads][page_size][64]``, changed in place.  Returns the new lengths ``ctx_len + n_accept``
-    (a negative ``ctx_len`` stays)."""
+    are).  ``n_accept`` must not pass the rows that were planned.  Caches ``[n_layers][n_pages][kv_heads][page_size][64]``, changed in place.
+    Returns the new lengths ``ctx_len + n_accept`` (a negative ``ctx_len`` stays)."""
     return _S.kv_commit(k_cache, v_cache, block_table, ctx_len, path, n_accept)
