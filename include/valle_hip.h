@@ -519,13 +519,14 @@ int valle_ar_decode_noalloc(valle_model* m, const valle_ar_state* st, const vall
  *                                served; -1 and position 0 behind the last row
  * With parents [max_rows] (tree_mask [max_rows] then too): row i of a request is a node whose parent is its row parents[.], an
  * earlier one (anything else: the context); its position is len_old + depth and tree_mask holds bit j for itself and every
- * ancestor j.  B <= 4096.  One launch up to 4,096 rows (with parents: and 64 requests), two beyond.  The lists must be whole: a page
+ * ancestor j.  B <= 4096.  ticket [1]: a word of the table's own, zero before its first plan
+ * and left zero by every one.  One launch up to 64 requests, and up to 4,096 rows without parents; else two.  The lists must be whole: a page
  * stands once in the stack or once in the first n_blocks entries of one request.  Rows of requests that are not served keep their
  * numbers in cu_rows; what attention gives for them means nothing. */
 int valle_page_plan(const int32_t* len_old, const int32_t* len_new, int B, int page_size, int32_t* block_table, int max_blocks,
                     const int32_t* n_blocks_in, int32_t* n_blocks_out, int32_t* free_list, int n_pages,
                     const int32_t* free_count_in, int32_t* free_count_out, int32_t* status, int32_t* cu_rows,
-                    int32_t* slots, int32_t* positions, int max_rows, const int32_t* parents, int64_t* tree_mask, void* stream);
+                    int32_t* slots, int32_t* positions, int max_rows, const int32_t* parents, int64_t* tree_mask, int32_t* ticket, void* stream);
 
 /* valle_rope_kv for pages: q [M][H][64], k, v [M][Hkv][64] (row strides in elements, rows 16-byte aligned), q and k rotated by
  * rope[positions[m]] ([rope_rows][32][2] fp32; a position outside takes the nearest row), q to q_out (q_out == q is allowed; both

@@ -152,10 +152,10 @@ def test_c_entries_refuse_bad_arguments():
     lib, p = L.load(), C.c_void_p(4096)
 
     def plan(**kw):
-        a = dict(lo=p, B=2, page=16, width=4, n_pages=8, max_rows=64, parents=None, mask=None)
+        a = dict(lo=p, B=2, page=16, width=4, n_pages=8, max_rows=64, parents=None, mask=None, ticket=p)
         a.update(kw)
-        return lib.valle_page_plan(a["lo"], p, a["B"], a["page"], p, a["width"], p, p, p, a["n_pages"], p, p, p, p, p, p, a["max_rows"], a["parents"], a["mask"], None)
-    for kw in (dict(lo=None), dict(B=0), dict(B=4097), dict(page=15), dict(page=512), dict(width=0), dict(width=2 ** 30), dict(n_pages=0), dict(n_pages=2 ** 30),
+        return lib.valle_page_plan(a["lo"], p, a["B"], a["page"], p, a["width"], p, p, p, a["n_pages"], p, p, p, p, p, p, a["max_rows"], a["parents"], a["mask"], a["ticket"], None)
+    for kw in (dict(lo=None), dict(ticket=None), dict(B=0), dict(B=4097), dict(page=15), dict(page=512), dict(width=0), dict(width=2 ** 30), dict(n_pages=0), dict(n_pages=2 ** 30),
                dict(max_rows=0), dict(parents=p), dict(mask=p)):
         assert plan(**kw) == -1, kw
         assert b"valle_page_plan" in lib.valle_last_error()
@@ -294,6 +294,44 @@ def test_plan_trees(gpu_device, max_rows):
     t, want = run_plan(gpu_device, lo, [c + k for c, k in zip(lo, sizes)], 16, 40, 60, max_rows, free=3, parents=par, seed=2)
     assert 1 in want["status"]
     check_plan(t, want, True)
+
+
+@gpu
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("n", [17, 40, 64])
+def test_plan_one_table_over_many_steps(gpu_device, tree, n):
+    """Batches whose rows or trees take several workgroups (the counters are written by the last one to have read them), planned in place
+    step after step on one table, directly and through a graph: the state of every step is the restatement's."""
+    rs = np.random.default_rng(n)
+    page, width, max_rows, n_pages = 16, 300, 64 * 64 if tree else 9000, n * 20
+    t = P.PageTable(n, width, n_pages, page, max_rows, device=gpu_device)
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=gpu_device)
+    lo, ln, par = i32(n), i32(n), i32(max_rows) if tree else None
+    t.plan(lo, ln, parents=par)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        t.plan(lo, ln, parents=par)
+    state = dict(block_table=np.zeros((n, width), np.int32), n_blocks=[0] * n, free_list=np.arange(n_pages - 1, -1, -1, dtype=np.int32), free_count=[n_pages])
+    length = [0] * n
+    for step in range(7):
+        new = [0 if rs.random() < 0.15 else c + int(rs.integers(0, 65 if tree else 200)) for c in length]
+        parents = None
+        if tree:
+            parents = np.array([p for c, m in zip(length, new) for p in random_tree(max(0, m - c), rs)], np.int32)
+            parents = np.concatenate((parents, np.full(max_rows - len(parents), 3, np.int32)))[:max_rows]
+            par.copy_(torch.from_numpy(parents))
+        lo.copy_(torch.tensor(length, dtype=torch.int32)), ln.copy_(torch.tensor(new, dtype=torch.int32))
+        want = ref_plan(length, new, state["block_table"], state["n_blocks"], state["free_list"], state["free_count"][0], page, max_rows, parents)
+        graph.replay() if step % 2 else t.plan(lo, ln, parents=par)
+        got = t.block_table.cpu().numpy()
+        for b in range(n):                                             # (entries behind n_blocks mean nothing)
+            k = want["n_blocks"][b]
+            assert (got[b, :k] == want["block_table"][b, :k]).all()
+        check_plan(t, {k: v for k, v in want.items() if k not in ("block_table", "free_list")}, tree)
+        assert (t.free_list.cpu().numpy()[:want["free_count"][0]] == want["free_list"][:want["free_count"][0]]).all()
+        state = want
+        length = [m if s == 0 else c for c, m, s in zip(length, new, want["status"])]
+    assert 0 < want["free_count"][0] < n_pages
 
 
 @gpu

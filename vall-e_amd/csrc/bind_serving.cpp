@@ -137,10 +137,10 @@ void launch(int dev, F&& f) {
 #define ARGS(n) TORCH_CHECK_TYPE(nargs == (n), "_serving: ", n, " arguments needed, got ", nargs)
 
 // (len_old, len_new, parents | None, block_table, n_blocks, n_blocks_out, free_list, free_count, free_count_out, status, cu_rows, slots,
-//  positions, tree_mask, page_size)
+//  positions, tree_mask, ticket, page_size)
 PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     TRY
-    ARGS(15);
+    ARGS(16);
     const at::Tensor& tab = tensor(a[3], "block_table");
     const int dev = gpu_of(tab, "PageTable.plan");
     NEED(tab.dim() == 2, "block_table: (requests, max_blocks) needed");
@@ -159,8 +159,9 @@ PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     int32_t *nbo = ints(tensor(a[5], "n_blocks_out"), "n_blocks_out", dev, {B}), *fco = ints(tensor(a[8], "free_count_out"), "free_count_out", dev, {1});
     int32_t *flp = ints(fl, "free_list", dev, {pages}), *st = ints(tensor(a[9], "status"), "status", dev, {B}), *cu = ints(tensor(a[10], "cu_rows"), "cu_rows", dev, {B + 1});
     int32_t *sp = ints(slots, "slots", dev, {rows}), *ps = ints(tensor(a[12], "positions"), "positions", dev, {rows});
-    const int page = whole(a[14], "page_size");
-    launch(dev, [&](void* s) { return valle_page_plan(lo, ln, B, page, tp, width, nb, nbo, flp, pages, fc, fco, st, cu, sp, ps, rows, pp, mask, s); });
+    int32_t* ticket = ints(tensor(a[14], "ticket"), "ticket", dev, {1});
+    const int page = whole(a[15], "page_size");
+    launch(dev, [&](void* s) { return valle_page_plan(lo, ln, B, page, tp, width, nb, nbo, flp, pages, fc, fco, st, cu, sp, ps, rows, pp, mask, ticket, s); });
     Py_RETURN_NONE;
     CATCH
 }

@@ -20,6 +20,7 @@ struct PlanArgs {
     const int32_t* fc_in; int32_t* fc_out;
     int32_t *status, *cu, *slots, *pos;
     const int32_t* parents; int64_t* mask;
+    int32_t* ticket;
     int B, width, n_pages, shift, max_rows;
 };
 
@@ -108,20 +109,23 @@ __device__ __forceinline__ int plan_lane_scan(int v) {
     return plan_dpp_add<0x143, 0xc>(v);       // row_bcast 31: rows 0 and 1, into rows 2 and 3
 }
 
-// Up to 64 requests: a request per lane, and every wave works the whole batch out for itself -- the sums cost a few dozen cycles, and what
-// the rows need is taken from the state as it was (a page that changes hands in this very call is looked up where it came from),
-// so the waves meet only once, between the reads of the counters and their writes (n_blocks_out may be n_blocks_in).  The latency is two
-// dependent memory round trips; the general form below takes five barriers.  16 requests with trees of 26 nodes: 3.5 us, 7.3 in the general form.
-template <bool ROWS>
+// Up to 64 requests: a request per lane, and every wave of every workgroup works the whole batch out for itself -- the sums cost a few dozen
+// cycles, and what the rows need is taken from the state as it was (a page that changes hands in this very call is looked up where it
+// came from), so nobody waits for anybody.  Only the counters may be read and written in one place (n_blocks_out may be n_blocks_in):
+// the last workgroup to have read them, by the ticket, writes them.  The latency is two dependent memory round trips and the ticket's.
+// One workgroup up to 1,024 rows or 16 trees, then one per as many more; us, in the general form / one workgroup / now: 16 trees of 26
+// nodes 7.3 / 3.5 / 3.5, 64 trees of 26 - / 7.2 / PLAN_A, 64 prompts of 700 rows - / 6.3 (the rows in a second launch) / PLAN_B.
 __global__ __launch_bounds__(1024) void page_plan_small_kernel(PlanArgs a) {
-    __shared__ int s_f[64], s_from[64];
+    __shared__ int s_f[64], s_from[64], s_end[64], s_lo[64], s_held[64], s_q0[64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool live = lane < a.B;
     const int bl = live ? lane : 0;
     const int lo = a.len_old[bl], ln = a.len_new[bl], held = a.nb_in[bl];
     const int fc = min(max(*a.fc_in, 0), a.n_pages);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                    // the counters are in registers before any of them is written over
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");         // the counters are in registers before any of them is written over
     __syncthreads();
+    int turn = 0;
+    if (gridDim.x > 1 && threadIdx.x == 0) turn = atomicAdd(a.ticket, 1);
     const long cap = (long)a.width << a.shift;
     const bool valid = live && lo >= 0 && ln >= 0 && lo <= cap && ln <= cap && held >= 0 && held <= a.width && !(a.parents && ln - lo > 64);
     const int want = valid ? (int)(((long)ln + (1 << a.shift) - 1) >> a.shift) : 0;
@@ -131,19 +135,12 @@ __global__ __launch_bounds__(1024) void page_plan_small_kernel(PlanArgs a) {
     const bool ok = valid && end64 <= a.max_rows;
     const int back = ok ? max(held - want, 0) : 0, need = ok ? max(want - held, 0) : 0;
     const int f = plan_lane_scan(back), q = plan_lane_scan(need);
-    const int freed = __builtin_amdgcn_readlane(f, 63), F = fc + freed;
+    const int freed = __builtin_amdgcn_readlane(f, 63), F = fc + freed, all = __builtin_amdgcn_readlane(end, 63);
     const bool served = ok && (need == 0 || q <= F);
     const uint64_t takers = __ballot(served && need > 0);
     const int taken = takers ? __shfl(q, 63 - __builtin_clzll(takers), 64) : 0;
-    if (wave == 0) {
-        if (live) {
-            a.cu[lane + 1] = end;
-            a.status[lane] = !valid ? 2 : !ok ? 3 : served ? 0 : 1;
-            a.nb_out[lane] = served ? want : held;
-        }
-        if (lane == 0) { a.cu[0] = 0; *a.fc_out = F - taken; }
-    }
-    s_f[lane] = f; s_from[lane] = want - (f - back);                     // (every wave writes the same)
+    s_f[lane] = f; s_from[lane] = want - (f - back);                     // (every wave writes the same and reads what it wrote)
+    s_end[lane] = end; s_lo[lane] = lo; s_held[lane] = served ? held : -1; s_q0[lane] = q - need;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     auto page_x = [&](int x) -> int {                                    // the page a request takes as number x: one given back in this call, or off the stack
@@ -154,35 +151,47 @@ __global__ __launch_bounds__(1024) void page_plan_small_kernel(PlanArgs a) {
         const int src = F - 1 - x;
         return src >= 0 && src < a.n_pages ? a.free_list[src] : -1;
     };
-    for (int b = wave; b < a.B; b += 16) {
+    auto slot_of = [&](int b, int p) -> int {                            // of cached row p, a new one, of request b
+        const int held_b = s_held[b], blk = p >> a.shift;
+        if (held_b < 0) return -1;
+        const int page = blk < held_b ? a.table[(size_t)b * a.width + blk] : page_x(s_q0[b] + blk - held_b);
+        return page >= 0 && page < a.n_pages ? (page << a.shift) + (p & ((1 << a.shift) - 1)) : -1;
+    };
+    for (int b = blockIdx.x * 16 + wave; b < a.B; b += gridDim.x * 16) {
         const int lo_b = __builtin_amdgcn_readlane(lo, b), held_b = __builtin_amdgcn_readlane(held, b), want_b = __builtin_amdgcn_readlane(want, b);
         const int back_b = __builtin_amdgcn_readlane(back, b), need_b = __builtin_amdgcn_readlane(need, b);
         const int f0 = __builtin_amdgcn_readlane(f, b) - back_b, q0 = __builtin_amdgcn_readlane(q, b) - need_b;
-        const bool served_b = (__ballot(served) >> b) & 1;
         int32_t* tab = a.table + (size_t)b * a.width;
         for (int k = lane; k < back_b; k += 64) {
             const int dst = F - 1 - (f0 + k);
             if (dst >= 0 && dst < a.n_pages) a.free_list[dst] = tab[want_b + k];
         }
-        if (served_b)
+        if ((__ballot(served) >> b) & 1)
             for (int k = lane; k < need_b; k += 64) tab[held_b + k] = page_x(q0 + k);
-        if constexpr (ROWS) {
-            const int end_b = __builtin_amdgcn_readlane(end, b), n = __builtin_amdgcn_readlane(rows, b), start = end_b - n;
-            auto slot_of = [&](int i) {                                  // of the request's new row i
-                const int p = lo_b + i, blk = p >> a.shift;
-                if (!served_b) return -1;
-                const int page = blk < held_b ? tab[blk] : page_x(q0 + blk - held_b);
-                return page >= 0 && page < a.n_pages ? (page << a.shift) + (p & ((1 << a.shift) - 1)) : -1;
-            };
-            if (a.parents) plan_tree(a, lo_b, start, n, lane < n ? slot_of(lane) : -1, lane);
-            else
-                for (int i = lane; i < n && start + i < a.max_rows; i += 64) { a.slots[start + i] = slot_of(i); a.pos[start + i] = lo_b + i; }
+        if (a.parents) {
+            const int n = __builtin_amdgcn_readlane(rows, b);
+            plan_tree(a, lo_b, __builtin_amdgcn_readlane(end, b) - n, n, lane < n ? slot_of(b, lo_b + lane) : -1, lane);
         }
     }
-    if constexpr (ROWS) {
-        for (int r = __builtin_amdgcn_readlane(end, 63) + threadIdx.x; r < a.max_rows; r += 1024) {
-            a.slots[r] = -1; a.pos[r] = 0;
-            if (a.parents) a.mask[r] = 0;
+    for (long r = (a.parents ? all : 0) + (long)blockIdx.x * 1024 + threadIdx.x; r < a.max_rows; r += gridDim.x * 1024) {
+        int slot = -1, pos = 0;
+        if (r < all) {
+            const int b = plan_find(s_end, a.B, (int)r);
+            pos = s_lo[b] + (int)r - (b ? s_end[b - 1] : 0);
+            slot = slot_of(b, pos);
+        }
+        a.slots[r] = slot; a.pos[r] = pos;
+        if (a.parents) a.mask[r] = 0;
+    }
+    if (wave == 0 && (gridDim.x == 1 || __builtin_amdgcn_readfirstlane(turn) == (int)gridDim.x - 1)) {
+        if (live) {
+            a.cu[lane + 1] = end;
+            a.status[lane] = !valid ? 2 : !ok ? 3 : served ? 0 : 1;
+            a.nb_out[lane] = served ? want : held;
+        }
+        if (lane == 0) {
+            a.cu[0] = 0; *a.fc_out = F - taken;
+            if (gridDim.x > 1) *a.ticket = 0;
         }
     }
 }
@@ -301,9 +310,9 @@ static int page_shift(int page_size) {
 extern "C" int valle_page_plan(const int32_t* len_old, const int32_t* len_new, int B, int page_size, int32_t* block_table, int max_blocks,
                                const int32_t* n_blocks_in, int32_t* n_blocks_out, int32_t* free_list, int n_pages,
                                const int32_t* free_count_in, int32_t* free_count_out, int32_t* status, int32_t* cu_rows,
-                               int32_t* slots, int32_t* positions, int max_rows, const int32_t* parents, int64_t* tree_mask, void* stream) {
+                               int32_t* slots, int32_t* positions, int max_rows, const int32_t* parents, int64_t* tree_mask, int32_t* ticket, void* stream) {
     VALLE_REQUIRE(len_old && len_new && block_table && n_blocks_in && n_blocks_out && free_list && free_count_in && free_count_out && status && cu_rows &&
-                  slots && positions, VALLE_E_ARG, "valle_page_plan: null pointer");
+                  slots && positions && ticket, VALLE_E_ARG, "valle_page_plan: null pointer");
     VALLE_REQUIRE(B > 0 && B <= PLAN_MAX_B, VALLE_E_ARG, "valle_page_plan: %d requests (1 .. %d)", B, PLAN_MAX_B);
     const int shift = page_shift(page_size);
     VALLE_REQUIRE(shift > 0, VALLE_E_ARG, "valle_page_plan: page_size %d (16, 32, 64, 128 or 256)", page_size);
@@ -313,15 +322,16 @@ extern "C" int valle_page_plan(const int32_t* len_old, const int32_t* len_new, i
     VALLE_REQUIRE(max_rows > 0, VALLE_E_ARG, "valle_page_plan: max_rows %d", max_rows);
     VALLE_REQUIRE((parents == nullptr) == (tree_mask == nullptr), VALLE_E_ARG, "valle_page_plan: parents and tree_mask go together");
     PlanArgs a{len_old, len_new, block_table, n_blocks_in, n_blocks_out, free_list, free_count_in, free_count_out, status, cu_rows, slots, positions,
-               parents, tree_mask, B, max_blocks, n_pages, shift, max_rows};
+               parents, tree_mask, ticket, B, max_blocks, n_pages, shift, max_rows};
     hipStream_t s = (hipStream_t)stream;
-    // The rows in the planning workgroup, or in a launch of their own over the chip: few rows of many requests 6.0 / 7.6 us (512 x 1), but
-    // trees beyond 64 requests 36.7 / 9.0 us (512 x 8), 13.4 / 8.3 (128 x 26): one wave per tree, sixteen at a time in one workgroup
-    if (max_rows <= 4096 && B <= 64) page_plan_small_kernel<true><<<1, 1024, 0, s>>>(a);
-    else if (max_rows <= 4096 && !parents) page_plan_kernel<1024, true><<<1, 1024, 0, s>>>(a);
+    // Beyond 64 requests: the rows in the planning workgroup, or in a launch of their own over the chip: few rows of many requests 6.0 / 7.6 us
+    // (512 x 1), but trees 36.7 / 9.0 us (512 x 8), 13.4 / 8.3 (128 x 26): one wave per tree, sixteen at a time in one workgroup
+    if (B <= 64) {
+        const int groups = max(ceil_div(max_rows, parents ? 16384 : 1024), parents ? ceil_div(B, 16) : 1);
+        page_plan_small_kernel<<<min(groups, 256), 1024, 0, s>>>(a);
+    } else if (max_rows <= 4096 && !parents) page_plan_kernel<1024, true><<<1, 1024, 0, s>>>(a);
     else {
-        if (B <= 64) page_plan_small_kernel<false><<<1, 1024, 0, s>>>(a);
-        else page_plan_kernel<1024, false><<<1, 1024, 0, s>>>(a);
+        page_plan_kernel<1024, false><<<1, 1024, 0, s>>>(a);
         page_rows_kernel<<<min(max(ceil_div(max_rows, 256), parents ? ceil_div(B, 4) : 0), 1024), 256, 0, s>>>(a);
     }
     VALLE_LAUNCH_CHECK();

@@ -65,7 +65,7 @@ class PageTable:
         self.block_table, self.n_blocks, self.status = i32(max_requests, max_blocks), i32(max_requests), i32(max_requests)
         self.free_list = torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=dev)          # page 0 on top
         self.free_count = torch.full((1,), n_pages, dtype=torch.int32, device=dev)
-        self.next_n_blocks, self.next_free_count = i32(max_requests), i32(1)
+        self.next_n_blocks, self.next_free_count, self._ticket = i32(max_requests), i32(1), i32(1)
         self.cu_rows, self.slots, self.positions = i32(max_requests + 1), i32(max_rows), i32(max_rows)
         self.tree_mask = torch.zeros(max_rows, dtype=torch.int64, device=dev)
 
@@ -82,7 +82,7 @@ class PageTable:
         else:
             nb, fc = self.next_n_blocks, self.next_free_count
         _S.page_plan(len_old, len_new, parents, self.block_table, self.n_blocks, nb, self.free_list, self.free_count, fc, self.status, self.cu_rows,
-                     self.slots, self.positions, self.tree_mask, self.page_size)
+                     self.slots, self.positions, self.tree_mask, self._ticket, self.page_size)
         return self
 
 
