@@ -520,7 +520,7 @@ int valle_ar_decode_noalloc(valle_model* m, const valle_ar_state* st, const vall
  * With parents [max_rows] (tree_mask [max_rows] then too): row i of a request is a node whose parent is its row parents[.], an
  * earlier one (anything else: the context); its position is len_old + depth and tree_mask holds bit j for itself and every
  * ancestor j.  B <= 4096.  ticket [1]: a word of the table's own, zero before its first plan
- * and left zero by every one.  One launch up to 64 requests, and up to 4,096 rows without parents; else two.  The lists must be whole: a page
+ * and left zero by every one.  One launch up to 512 requests, and up to 4,096 rows without parents; else two.  The lists must be whole: a page
  * stands once in the stack or once in the first n_blocks entries of one request.  Rows of requests that are not served keep their
  * numbers in cu_rows; what attention gives for them means nothing. */
 int valle_page_plan(const int32_t* len_old, const int32_t* len_new, int B, int page_size, int32_t* block_table, int max_blocks,

@@ -298,12 +298,12 @@ def test_plan_trees(gpu_device, max_rows):
 
 @gpu
 @pytest.mark.parametrize("tree", [False, True])
-@pytest.mark.parametrize("n", [17, 40, 64])
+@pytest.mark.parametrize("n", [17, 40, 64, 65, 200, 512, 600])
 def test_plan_one_table_over_many_steps(gpu_device, tree, n):
     """Batches whose rows or trees take several workgroups (the counters are written by the last one to have read them), planned in place
     step after step on one table, directly and through a graph: the state of every step is the restatement's."""
     rs = np.random.default_rng(n)
-    page, width, max_rows, n_pages = 16, 300, 64 * 64 if tree else 9000, n * 20
+    page, width, max_rows, n_pages = 16, 300, n * 64 if tree else n * 140, n * 20
     t = P.PageTable(n, width, n_pages, page, max_rows, device=gpu_device)
     i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=gpu_device)
     lo, ln, par = i32(n), i32(n), i32(max_rows) if tree else None

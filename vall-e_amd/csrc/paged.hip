@@ -109,40 +109,82 @@ __device__ __forceinline__ int plan_lane_scan(int v) {
     return plan_dpp_add<0x143, 0xc>(v);       // row_bcast 31: rows 0 and 1, into rows 2 and 3
 }
 
-// Up to 64 requests: a request per lane, and every wave of every workgroup works the whole batch out for itself -- the sums cost a few dozen
-// cycles, and what the rows need is taken from the state as it was (a page that changes hands in this very call is looked up where it
+// Up to 64 E requests, E neighbours per lane of a wave.  Every workgroup works the whole batch out for itself (at E = 1 every wave: the sums cost
+// a few dozen cycles; beyond, its first wave, between two barriers), and what the rows need is taken from the state as it was (a page that changes hands in this very call is looked up where it
 // came from), so nobody waits for anybody.  Only the counters may be read and written in one place (n_blocks_out may be n_blocks_in):
 // the last workgroup to have read them, by the ticket, writes them.  The latency is two dependent memory round trips and the ticket's.
-// One workgroup up to 1,024 rows or 16 trees, then one per as many more; us, in the general form / one workgroup / now: 16 trees of 26
-// nodes 7.3 / 3.5 / 3.5, 64 trees of 26 - / 7.2 / PLAN_A, 64 prompts of 700 rows - / 6.3 (the rows in a second launch) / PLAN_B.
-__global__ __launch_bounds__(1024) void page_plan_small_kernel(PlanArgs a) {
-    __shared__ int s_f[64], s_from[64], s_end[64], s_lo[64], s_held[64], s_q0[64];
+// One workgroup up to 1,024 rows or 16 trees, then one per as many more; us, in the general form / in one workgroup / now: 16 trees of 26
+// nodes 7.3 / 3.5 / 3.6, 64 trees of 26 - / 7.2 / 3.8, 64 prompts of 700 rows - / 6.3 (their rows in a second launch) / 3.9; with E = 8
+// 128 trees of 26 8.3 / - / 5.8, 512 of 8 9.0 / - / 6.3, 512 requests with a row each 6.0 / - / 5.1 (every wave for itself there too: 9.7, 17, 22).
+template <int E>
+__global__ __launch_bounds__(1024) void page_plan_wave_kernel(PlanArgs a) {
+    __shared__ int s_f[64 * E], s_from[64 * E], s_end[64 * E], s_lo[64 * E], s_held[64 * E], s_q[64 * E], s_sum[2];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const bool live = lane < a.B;
-    const int bl = live ? lane : 0;
-    const int lo = a.len_old[bl], ln = a.len_new[bl], held = a.nb_in[bl];
+    int lo[E], ln[E], held[E];
+    if constexpr (E == 1) {
+        const int b = min(lane, a.B - 1);
+        lo[0] = a.len_old[b]; ln[0] = a.len_new[b]; held[0] = a.nb_in[b];
+    } else if (threadIdx.x < 64 * E) {                                   // whole lines, for the first wave
+        const int b = min((int)threadIdx.x, a.B - 1);
+        s_lo[threadIdx.x] = a.len_old[b]; s_f[threadIdx.x] = a.len_new[b]; s_held[threadIdx.x] = a.nb_in[b];
+    }
     const int fc = min(max(*a.fc_in, 0), a.n_pages);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");         // the counters are in registers before any of them is written over
     __syncthreads();
     int turn = 0;
     if (gridDim.x > 1 && threadIdx.x == 0) turn = atomicAdd(a.ticket, 1);
     const long cap = (long)a.width << a.shift;
-    const bool valid = live && lo >= 0 && ln >= 0 && lo <= cap && ln <= cap && held >= 0 && held <= a.width && !(a.parents && ln - lo > 64);
-    const int want = valid ? (int)(((long)ln + (1 << a.shift) - 1) >> a.shift) : 0;
-    const int rows = valid && ln > lo ? ln - lo : 0;
-    const long end64 = (long)plan_lane_scan(rows & 0xffff) + ((long)plan_lane_scan(rows >> 16) << 16);
-    const int end = (int)min(end64, (long)INT32_MAX);
-    const bool ok = valid && end64 <= a.max_rows;
-    const int back = ok ? max(held - want, 0) : 0, need = ok ? max(want - held, 0) : 0;
-    const int f = plan_lane_scan(back), q = plan_lane_scan(need);
-    const int freed = __builtin_amdgcn_readlane(f, 63), F = fc + freed, all = __builtin_amdgcn_readlane(end, 63);
-    const bool served = ok && (need == 0 || q <= F);
-    const uint64_t takers = __ballot(served && need > 0);
-    const int taken = takers ? __shfl(q, 63 - __builtin_clzll(takers), 64) : 0;
-    s_f[lane] = f; s_from[lane] = want - (f - back);                     // (every wave writes the same and reads what it wrote)
-    s_end[lane] = end; s_lo[lane] = lo; s_held[lane] = served ? held : -1; s_q0[lane] = q - need;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    int want[E], rows[E], f[E], q[E], end[E], freed = 0, F = 0, all = 0, taken = 0;
+    bool valid[E], ok[E], served[E];
+    if (E == 1 || wave == 0) {
+        if constexpr (E > 1) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) { lo[e] = s_lo[lane * E + e]; ln[e] = s_f[lane * E + e]; held[e] = s_held[lane * E + e]; }
+        }
+        int low = 0, high = 0, gone = 0, asked = 0;                          // of the lane's requests: rows (16 bits and the rest), pages back, pages asked for
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            valid[e] = lane * E + e < a.B && lo[e] >= 0 && ln[e] >= 0 && lo[e] <= cap && ln[e] <= cap && held[e] >= 0 && held[e] <= a.width && !(a.parents && ln[e] - lo[e] > 64);
+            want[e] = valid[e] ? (int)(((long)ln[e] + (1 << a.shift) - 1) >> a.shift) : 0;
+            rows[e] = valid[e] && ln[e] > lo[e] ? ln[e] - lo[e] : 0;
+            low += rows[e] & 0xffff; high += rows[e] >> 16;
+        }
+        long at = (long)plan_lane_scan(low) - low + ((long)(plan_lane_scan(high) - high) << 16);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            at += rows[e];
+            end[e] = (int)min(at, (long)INT32_MAX);
+            ok[e] = valid[e] && at <= a.max_rows;
+            f[e] = gone += ok[e] ? max(held[e] - want[e], 0) : 0;
+            q[e] = asked += ok[e] ? max(want[e] - held[e], 0) : 0;
+        }
+        const int f_all = plan_lane_scan(gone), q_all = plan_lane_scan(asked);
+        freed = __builtin_amdgcn_readlane(f_all, 63); F = fc + freed; all = __builtin_amdgcn_readlane(end[E - 1], 63);
+        int last = 0;                                                        // pages taken up to the lane's last served request that takes some
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int need = ok[e] ? max(want[e] - held[e], 0) : 0;
+            f[e] += f_all - gone; q[e] += q_all - asked;
+            served[e] = ok[e] && (need == 0 || q[e] <= F);
+            if (served[e] && need > 0) last = q[e];
+        }
+        const uint64_t takers = __ballot(last > 0);
+        taken = takers ? __shfl(last, 63 - __builtin_clzll(takers), 64) : 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {                                    // (E == 1: every wave writes the same and reads what it wrote)
+            const int b = lane * E + e;
+            s_f[b] = f[e]; s_from[b] = want[e] - f[e] + (ok[e] ? max(held[e] - want[e], 0) : 0);
+            s_end[b] = end[e]; s_lo[b] = lo[e]; s_held[b] = served[e] ? held[e] : -1; s_q[b] = q[e];
+        }
+    }
+    if constexpr (E == 1) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    } else {
+        if (threadIdx.x == 0) { s_sum[0] = freed; s_sum[1] = all; }
+        __syncthreads();
+        freed = s_sum[0]; all = s_sum[1]; F = fc + freed;
+    }
     auto page_x = [&](int x) -> int {                                    // the page a request takes as number x: one given back in this call, or off the stack
         if (x < freed) {
             const int b = plan_find(s_f, a.B, x);
@@ -154,23 +196,21 @@ __global__ __launch_bounds__(1024) void page_plan_small_kernel(PlanArgs a) {
     auto slot_of = [&](int b, int p) -> int {                            // of cached row p, a new one, of request b
         const int held_b = s_held[b], blk = p >> a.shift;
         if (held_b < 0) return -1;
-        const int page = blk < held_b ? a.table[(size_t)b * a.width + blk] : page_x(s_q0[b] + blk - held_b);
+        const int page = blk < held_b ? a.table[(size_t)b * a.width + blk] : page_x((b ? s_q[b - 1] : 0) + blk - held_b);
         return page >= 0 && page < a.n_pages ? (page << a.shift) + (p & ((1 << a.shift) - 1)) : -1;
     };
     for (int b = blockIdx.x * 16 + wave; b < a.B; b += gridDim.x * 16) {
-        const int lo_b = __builtin_amdgcn_readlane(lo, b), held_b = __builtin_amdgcn_readlane(held, b), want_b = __builtin_amdgcn_readlane(want, b);
-        const int back_b = __builtin_amdgcn_readlane(back, b), need_b = __builtin_amdgcn_readlane(need, b);
-        const int f0 = __builtin_amdgcn_readlane(f, b) - back_b, q0 = __builtin_amdgcn_readlane(q, b) - need_b;
+        const int f0 = b ? s_f[b - 1] : 0, back = s_f[b] - f0, q0 = b ? s_q[b - 1] : 0, need = s_q[b] - q0, held_b = s_held[b];
         int32_t* tab = a.table + (size_t)b * a.width;
-        for (int k = lane; k < back_b; k += 64) {
+        for (int k = lane; k < back; k += 64) {
             const int dst = F - 1 - (f0 + k);
-            if (dst >= 0 && dst < a.n_pages) a.free_list[dst] = tab[want_b + k];
+            if (dst >= 0 && dst < a.n_pages) a.free_list[dst] = tab[s_from[b] + f0 + k];
         }
-        if ((__ballot(served) >> b) & 1)
-            for (int k = lane; k < need_b; k += 64) tab[held_b + k] = page_x(q0 + k);
+        if (held_b >= 0)
+            for (int k = lane; k < need; k += 64) tab[held_b + k] = page_x(q0 + k);
         if (a.parents) {
-            const int n = __builtin_amdgcn_readlane(rows, b);
-            plan_tree(a, lo_b, __builtin_amdgcn_readlane(end, b) - n, n, lane < n ? slot_of(b, lo_b + lane) : -1, lane);
+            const int start = b ? s_end[b - 1] : 0, n = s_end[b] - start;
+            plan_tree(a, s_lo[b], start, n, lane < n ? slot_of(b, s_lo[b] + lane) : -1, lane);
         }
     }
     for (long r = (a.parents ? all : 0) + (long)blockIdx.x * 1024 + threadIdx.x; r < a.max_rows; r += gridDim.x * 1024) {
@@ -184,10 +224,14 @@ __global__ __launch_bounds__(1024) void page_plan_small_kernel(PlanArgs a) {
         if (a.parents) a.mask[r] = 0;
     }
     if (wave == 0 && (gridDim.x == 1 || __builtin_amdgcn_readfirstlane(turn) == (int)gridDim.x - 1)) {
-        if (live) {
-            a.cu[lane + 1] = end;
-            a.status[lane] = !valid ? 2 : !ok ? 3 : served ? 0 : 1;
-            a.nb_out[lane] = served ? want : held;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int b = lane * E + e;
+            if (b < a.B) {
+                a.cu[b + 1] = end[e];
+                a.status[b] = !valid[e] ? 2 : !ok[e] ? 3 : served[e] ? 0 : 1;
+                a.nb_out[b] = served[e] ? want[e] : held[e];
+            }
         }
         if (lane == 0) {
             a.cu[0] = 0; *a.fc_out = F - taken;
@@ -196,7 +240,7 @@ __global__ __launch_bounds__(1024) void page_plan_small_kernel(PlanArgs a) {
     }
 }
 
-// One workgroup plans the batch, five rounds of barriers (512 requests, a row each: 6.0 us; 4,096: 14) (a request per thread, up to four); ROWS: it also fills the rows (no trees), else page_rows_kernel does.
+// One workgroup plans the batch, five rounds of barriers (4,096 requests, a row each: 14 us) (a request per thread, up to four); ROWS: it also fills the rows (no trees), else page_rows_kernel does.
 template <int NT, bool ROWS>
 __global__ __launch_bounds__(NT) void page_plan_kernel(PlanArgs a) {
     constexpr int E = 4;
@@ -324,11 +368,11 @@ extern "C" int valle_page_plan(const int32_t* len_old, const int32_t* len_new, i
     PlanArgs a{len_old, len_new, block_table, n_blocks_in, n_blocks_out, free_list, free_count_in, free_count_out, status, cu_rows, slots, positions,
                parents, tree_mask, ticket, B, max_blocks, n_pages, shift, max_rows};
     hipStream_t s = (hipStream_t)stream;
-    // Beyond 64 requests: the rows in the planning workgroup, or in a launch of their own over the chip: few rows of many requests 6.0 / 7.6 us
-    // (512 x 1), but trees 36.7 / 9.0 us (512 x 8), 13.4 / 8.3 (128 x 26): one wave per tree, sixteen at a time in one workgroup
-    if (B <= 64) {
-        const int groups = max(ceil_div(max_rows, parents ? 16384 : 1024), parents ? ceil_div(B, 16) : 1);
-        page_plan_small_kernel<<<min(groups, 256), 1024, 0, s>>>(a);
+    // Beyond 512 requests: the rows in the planning workgroup, or in a launch of their own over the chip, trees always (512 x 8: 36.7 / 9.0 us)
+    if (B <= 512) {
+        const int groups = min(max(ceil_div(max_rows, parents ? 16384 : 1024), parents || B > 64 ? ceil_div(B, 16) : 1), 256);
+        if (B <= 64) page_plan_wave_kernel<1><<<groups, 1024, 0, s>>>(a);
+        else page_plan_wave_kernel<8><<<groups, 1024, 0, s>>>(a);
     } else if (max_rows <= 4096 && !parents) page_plan_kernel<1024, true><<<1, 1024, 0, s>>>(a);
     else {
         page_plan_kernel<1024, false><<<1, 1024, 0, s>>>(a);
