@@ -67,6 +67,16 @@ def test_quantize_w4_is_within_half_a_step():
         assert ((back - w.double()).abs() <= slack * step * (1 + 1e-6) + 1e-9).all()
 
 
+def test_quantize_w4_refuses_what_has_no_four_bits():
+    for w, group in ((torch.randn(4, 100), 64), (torch.full((4, 64), float("nan")), 64), (torch.full((4, 64), float("inf")), 32)):
+        with pytest.raises(ValueError):
+            PL.quantize_w4(w, group)
+    with pytest.raises(ValueError):
+        PL.HipLinear4(64, 4).load_state_dict({"weight": torch.full((4, 64), float("nan")), "bias": torch.zeros(4)})
+    with pytest.raises(ValueError):
+        PL.HipLinear4(64, 4).load_state_dict({"weight": torch.zeros(4, 128), "bias": torch.zeros(4)})
+
+
 def test_packed_layout_holds_every_weight():
     """The documented layout, element by element."""
     n, k, group = 18, 160, 32

@@ -71,13 +71,14 @@ __device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[2][1]) {
     asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:1024\n\ts_waitcnt lgkmcnt(0)" : "=&v"(x[0][0]), "=&v"(x[1][0]) : "v"(at) : "memory");
 }
 __device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[2][2]) {
-    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\tds_read_b128 %2, %4 offset:2048\n\tds_read_b128 %3, %4 offset:3072\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1]) : "v"(at) : "memory");
+    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%5\n\tds_read_b128 %2, %4 offset:%6\n\tds_read_b128 %3, %4 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1]) : "v"(at), "n"(1 << 10), "n"(2 << 10), "n"(3 << 10) : "memory");
 }
 __device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[2][3]) {
-    asm volatile("ds_read_b128 %0, %6\n\tds_read_b128 %1, %6 offset:1024\n\tds_read_b128 %2, %6 offset:2048\n\tds_read_b128 %3, %6 offset:3072\n\t"
-                 "ds_read_b128 %4, %6 offset:4096\n\tds_read_b128 %5, %6 offset:5120\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[0][2]), "=&v"(x[1][0]), "=&v"(x[1][1]), "=&v"(x[1][2]) : "v"(at) : "memory");
+    asm volatile("ds_read_b128 %0, %6\n\tds_read_b128 %1, %6 offset:%7\n\tds_read_b128 %2, %6 offset:%8\n\tds_read_b128 %3, %6 offset:%9\n\t"
+                 "ds_read_b128 %4, %6 offset:%10\n\tds_read_b128 %5, %6 offset:%11\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[0][2]), "=&v"(x[1][0]), "=&v"(x[1][1]), "=&v"(x[1][2])
+                 : "v"(at), "n"(1 << 10), "n"(2 << 10), "n"(3 << 10), "n"(4 << 10), "n"(5 << 10) : "memory");
 }
 
 template <int G, int NT, int MT, int NW>

@@ -42,7 +42,8 @@ def kv_cache(n_layers, n_pages, page_size, kv_heads, dtype=torch.bfloat16, devic
 
 
 class PageTable:
-    """The pages of a batch of up to ``max_requests`` requests over a pool of ``n_pages``, kept on the device.
+    """The pages of a batch of up to ``max_requests`` requests over a pool of ``n_pages``, kept on the device.  One plan at a time: plans of
+    one table on two streams must wait for each other.
 
     State: ``block_table [max_requests][max_blocks]`` int32 (entries behind a request's ``n_blocks`` mean nothing), ``n_blocks``
     [max_requests], ``free_list`` [n_pages] (a stack of the first ``free_count[0]`` entries).

@@ -91,6 +91,8 @@ def quantize_w4(weight, group_size=64, symmetric=False):
     ``[out][in / 2]`` (two to a byte, the even input in the low nibble), scales ``[out][in / group]`` in the weight's type, zeros
     uint8 of the same shape (None when symmetric: 8)."""
     n, k = weight.shape
+    if k % group_size or not torch.isfinite(weight).all():
+        raise ValueError(f"quantize_w4: finite weights and a group_size that divides {k} needed (got {group_size})")
     w = weight.detach().float().reshape(n, k // group_size, group_size)
     if symmetric:
         s = (w.abs().amax(-1) / 7.0).to(weight.dtype).float()
