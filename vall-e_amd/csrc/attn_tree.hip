@@ -13,6 +13,8 @@
 // not faster: products placed between the exponentials by scheduling groups, one block's P.V delayed under the next one's exponentials,
 // two loops (with and without masks: spills), query groups of a workgroup sharing tiles.
 #include "common.h"
+#include <algorithm>
+#include <type_traits>
 
 struct TreeArgs {
     const void *q, *kc, *vc;
@@ -170,8 +172,11 @@ __device__ __forceinline__ void tree_clean_v(TreeTile<T>& t, int s, int r) {
         if (!(fabsf(to_f32<T>(t.v[s][r][e])) < INFINITY)) t.v[s][r][e] = from_f32<T>(0.f);
 }
 
+// waves per SIMD that the registers are held down to
+template <typename T> constexpr int tree_waves(int qb) { return qb == 4 ? 2 : qb == 2 ? 3 : sizeof(T) == 2 ? 4 : 3; }
+
 template <typename T, int QB, int NW>
-__global__ __launch_bounds__(NW * 64, QB == 1 && sizeof(T) == 2 ? 4 : 2) void attn_tree_kernel(TreeArgs a) {
+__global__ __launch_bounds__(NW * 64, tree_waves<T>(QB)) void attn_tree_kernel(TreeArgs a) {
     typedef TreeTile<T> Tile;
     constexpr int SUB = Tile::SUB, KT = 16 * SUB;
     const int split = blockIdx.x, kvh = blockIdx.y % a.Hkv, qblk = blockIdx.y / a.Hkv, b = blockIdx.z;
@@ -489,36 +494,61 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeArgs a) {
     ((T*)a.out)[row * a.o_rs + head * 64 + lane] = from_f32<T>(L == 0.f ? 0.f : acc / L);
 }
 
-// How the work is cut: qb blocks of 16 queries per wave (fp32 tiles leave registers for two), `blocks` workgroups over the queries of a
-// (request, kv head), `split` over its keys.  A block more per wave saves key traffic and a wave's K and V turns, but costs registers (four
-// waves per SIMD at one block, two beyond), a longer start and end, and workgroups; splitting fills the chip but needs the join.  The
-// estimate in 0.1 us is fitted to measurements (bf16 unless said; us at 1 / 2 / 4 blocks; requests x context, nodes, heads / kv heads):
-//   1 x 130,001, 64, 16/4: 121 / 83 / 69     16 x 2,000, 64, 16/4: 35 / 29 / 23      16 x 536, 64, 16/4: 16.4 / 15.7 / 12.9
-//   32 x 2,200, 64, 16/16: 96 / 79 / 62      64 x 536, 26, 16/16: 33 / 40            16 x 536, 16, 16/4: 6.3 / 8.2 / 11.6
-//   1 x 64, 64, 16/4: 4.6 / 6.3 / 8.9        32 x 2,200, 26, 16/16: 57 / 52          fp32 1 x 300, 64, 16/16: 8.5 / 13.3; 16 x 64, 64, 16/16: 18.8 / 17.0
-struct TreeShape { int qb, blocks, split; };
+// How the work is cut: qb blocks of 16 queries per wave (fp32 tiles leave registers for two), nw waves per workgroup over the keys, `blocks`
+// workgroups over the queries of a (request, kv head), `split` over its keys.  More blocks per wave save key traffic and the turning of K
+// and V, but hold more registers (four, three, two waves per SIMD at one, two, four blocks) and start and end longer; eight waves finish a
+// request sooner, workgroups of four overlap one's start and end with another's tiles; splitting fills the chip but needs the join.
+// The choice is the least of an estimate in us, fitted to 624 measurements of 33 shapes (it takes 1.3 % more than the best of them, in the
+// mean).  Some of them in bf16, us with qb x nw (requests x context, nodes, heads / kv heads):
+//                                  1 x 4   1 x 8   2 x 4   2 x 8   4 x 4   4 x 8
+//   1 x 130,001, 64, 16/4           114     111      75      74      66      64
+//   32 x 2,200, 64, 16/16            95      93      58      74      52      59
+//   32 x 2,200, 26, 16/16            56      55      46      51
+//   48 x 300, 64, 16/16              27      38      24      42      26      37
+//   16 x 536, 64, 16/4             14.0    16.5    11.2    15.8    12.3    12.8
+//   16 x 536, 26, 16/16             9.4    10.1     9.9     9.7
+//   1 x 300, 64, 16/16              5.5     5.7     7.0     7.4     9.9    10.6
+//   16 x 536, 1, 16/16              7.4     6.9
+// and in fp32: 64 x 536, 26, 16/16 65 / 85 / 57 / 75; 1 x 4,000, 26, 16/16 15 / 14 / 18 / 18.
+struct TreeShape { int qb, nw, blocks, split; };
+struct TreeCost {
+    float issue[3], tile[3];            // of one tile by qb: of the SIMD's issue slots, and of a wave alone
+    float ends[3], ends4;               // start and end of a workgroup of eight waves, and the factor for four
+    float join, part;                   // second launch (and 0.05 per part it joins); per MB of partial sums
+    float mem, again;                   // per MB of keys and values; share of it for every further workgroup that reads them
+    float both;                         // share of the shorter of compute and memory that is not hidden
+};
 static TreeShape tree_shape(int B, int Hkv, int g, int max_nodes, int max_ctx, int kt) {
-    const int nq = max_nodes * g, nw = 8;
+    static const TreeCost bf{{.354f, .432f, .684f}, {.55f, .69f, 1.02f}, {2.24f, 3.89f, 6.1f}, .79f, 2.6f, .26f, 1 / 7800.f, .08f, .43f};
+    static const TreeCost fp{{.496f, 1.048f, 0.f}, {.734f, 1.26f, 0.f}, {2.57f, 4.68f, 0.f}, .62f, 2.45f, .28f, 1 / 7400.f, .17f, .32f};
+    const bool bf16s = kt == 32;
+    const TreeCost& c = bf16s ? bf : fp;
+    const int nq = max_nodes * g;
     const long tiles = ((long)max_ctx + max_nodes + kt - 1) / kt;
-    TreeShape best{0, 0, 0};
-    double least = 0;
-    for (int qb = 1; qb <= (kt == 16 ? 2 : 4) && (qb == 1 || nq > 8 * qb); qb *= 2) {
+    const float kb = (float)B * Hkv * tiles * 8.192f;                     // a tile's K and V are 8 KB in either type
+    TreeShape best{0, 0, 0, 0};
+    float least = 0.f;
+    for (int q = 0; q < (bf16s ? 3 : 2) && (q == 0 || nq > 8 << q); ++q) {
+        const int qb = 1 << q;
         const long blocks = ceil_div(nq, 16 * qb), base = (long)B * Hkv * blocks;
         if (Hkv * blocks > 65535) continue;                              // (no such grid)
-        const long room = kt == 32 && qb == 1 ? 512 : 256;               // workgroups that run at a time
-        for (int whole = 1; whole >= 0; --whole) {
-            long split = whole ? 1 : room / base;
-            if (split > tiles / (2 * nw)) split = tiles / (2 * nw);      // (a wave keeps two tiles)
-            if (split > TREE_MAX_SPLIT) split = TREE_MAX_SPLIT;
-            if (split < 1 || (!whole && split == 1)) { if (!whole) continue; split = 1; }
-            const long groups = base * split, deep = (tiles + nw * split - 1) / (nw * split);
-            const double rounds = (double)((groups + room - 1) / room);
-            double t;
-            if (kt == 16) t = rounds * (qb == 1 ? 20 + 11.5 * deep : 40 + 22.0 * deep);
-            else if (qb == 1) t = groups <= 256 ? 8 + 8.0 * deep : rounds * (20 + 18.0 * deep);
-            else t = rounds * (qb == 2 ? 42 + 13.0 * deep : 50 + 18.0 * deep);
-            if (split > 1) t += 35 + (double)B * max_nodes * g * Hkv * split * 512 / 4e5;      // a launch, and the partial sums out and in at 4 TB/s
-            if (!best.qb || t < least) { best = TreeShape{qb, (int)blocks, (int)split}; least = t; }
+        const float mem = kb * c.mem * (1.f + c.again * (blocks - 1));
+        for (int nw = 8; nw >= 4; nw -= 4) {
+            const long room = 256 * ((q == 0 && bf16s ? 16 : q == 2 ? 8 : 12) / nw);       // workgroups at a time
+            const long most = std::min<long>(std::min<long>(room / base, TREE_MAX_SPLIT), tiles / (2 * nw));    // (a wave keeps two tiles)
+            long last = 0;
+            for (int part = 2; part >= 0; --part) {                      // one, half of the most, the most
+                const long split = part == 2 ? 1 : part == 1 ? most / 2 : most;
+                if (split <= last) continue;
+                last = split;
+                const long groups = base * split, rounds = (groups + room - 1) / room, deep = (tiles + nw * split - 1) / (nw * split);
+                const long per_cu = (std::min(groups, room) + 255) / 256;
+                const float tile = std::max(c.tile[q], c.issue[q] * (per_cu * nw * .25f));
+                const float work = rounds * (c.ends[q] * (nw == 4 ? c.ends4 : 1.f) + deep * tile);
+                float t = std::max(work, mem) + c.both * std::min(work, mem);
+                if (split > 1) t += c.join + .05f * split + c.part * ((float)B * nq * Hkv * split * 512e-6f);
+                if (!best.qb || t < least) { best = TreeShape{qb, nw, (int)blocks, (int)split}; least = t; }
+            }
         }
     }
     return best;
@@ -526,20 +556,25 @@ static TreeShape tree_shape(int B, int Hkv, int g, int max_nodes, int max_ctx, i
 static bool tree_shape_ok(int rows, int B, int H, int Hkv, int max_nodes, int max_ctx) {
     return rows >= 0 && B >= 0 && B <= 65535 && H > 0 && Hkv > 0 && H % Hkv == 0 && H <= 65535 && H / Hkv <= 1024 && max_nodes > 0 && max_nodes <= TREE_MAX_NODES && max_ctx >= 0;
 }
-#define TREE_NW 8
+
+static size_t tree_bytes(int rows, int H, int split) { return split <= 1 ? 0 : (size_t)rows * H * split * 66 * sizeof(float); }
 
 extern "C" size_t valle_attn_tree_workspace_bytes(int rows, int B, int max_nodes, int max_ctx, int H, int Hkv, int dtype) {
     if (!tree_shape_ok(rows, B, H, Hkv, max_nodes, max_ctx) || B == 0) return 0;
-    const int ns = tree_shape(B, Hkv, H / Hkv, max_nodes, max_ctx, dtype == VALLE_BF16 ? 32 : 16).split;
-    return ns <= 1 ? 0 : (size_t)rows * H * ns * 66 * sizeof(float);
+    return tree_bytes(rows, H, tree_shape(B, Hkv, H / Hkv, max_nodes, max_ctx, dtype == VALLE_BF16 ? 32 : 16).split);
 }
 
 template <typename T>
 static void tree_launch(const TreeArgs& a, const TreeShape& t, int B, hipStream_t s) {
     const dim3 grid(a.nsplit, a.Hkv * t.blocks, B);
-    if (t.qb == 1) attn_tree_kernel<T, 1, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
-    else if (t.qb == 2) attn_tree_kernel<T, 2, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
-    else if constexpr (sizeof(T) == 2) attn_tree_kernel<T, 4, TREE_NW><<<grid, TREE_NW * 64, 0, s>>>(a);
+    auto go = [&](auto qb, auto nw) { attn_tree_kernel<T, decltype(qb)::value, decltype(nw)::value><<<grid, decltype(nw)::value * 64, 0, s>>>(a); };
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    const std::integral_constant<int, 4> four;
+    const std::integral_constant<int, 8> eight;
+    if (t.qb == 1) t.nw == 8 ? go(one, eight) : go(one, four);
+    else if (t.qb == 2) t.nw == 8 ? go(two, eight) : go(two, four);
+    else if constexpr (sizeof(T) == 2) t.nw == 8 ? go(four, eight) : go(four, four);
     if (a.nsplit > 16) attn_tree_join_kernel<T, 4><<<dim3(B, a.max_nodes, a.H), 256, 0, s>>>(a);
     else if (a.nsplit > 1) attn_tree_join_kernel<T, 1><<<dim3(B, a.max_nodes, ceil_div(a.H, 4)), 256, 0, s>>>(a);
 }
@@ -571,7 +606,7 @@ extern "C" int valle_attn_tree(const void* q, int64_t q_row_stride, const void* 
                softmax_scale * 1.4426950408889634f, (uint32_t)(((1ull << 32) + H / Hkv - 1) / (H / Hkv)), max_blocks, n_pages, shift, rows, H, Hkv, H / Hkv, max_nodes, 1};
     const TreeShape shape = tree_shape(B, Hkv, a.g, max_nodes, max_ctx, dtype == VALLE_BF16 ? 32 : 16);
     a.nsplit = shape.split;
-    const size_t need = valle_attn_tree_workspace_bytes(rows, B, max_nodes, max_ctx, H, Hkv, dtype);
+    const size_t need = tree_bytes(rows, H, shape.split);
     VALLE_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), VALLE_E_WORKSPACE,
                   "valle_attn_tree: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
     VALLE_REQUIRE(shape.qb, VALLE_E_ARG, "valle_attn_tree: %d heads are too many", H);
