@@ -201,7 +201,8 @@ def test_linear_w4_replaces_nn_linear(gpu_device):
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows,n,k,group", [(1, 1000, 4096, 64), (1, 72, 8320, 128), (1, 4100, 2336, 32), (1, 4112, 1216, 64), (40, 8200, 1408, 128), (33, 8192, 1216, 64),
-                                            (20, 8192, 1184, 32), (7, 8194, 3264, 64), (48, 4096, 4224, 128), (97, 200, 1184, 32)])
+                                            (20, 8192, 1184, 32), (7, 8194, 3264, 64), (48, 4096, 4224, 128), (97, 200, 1184, 32),
+                                            (64, 8192, 1216, 64), (57, 8200, 1408, 128), (50, 8208, 2336, 32), (64, 8200, 992, 32), (120, 8256, 4224, 128)])
 def test_linear_w4_long_and_wide(gpu_device, dtype, rows, n, k, group):
     """Several k blocks per wave in every form: last blocks that are no whole ones, an odd number of them, columns behind the last tile."""
     q, s, z = make(n, k, group, True, dtype, n + k)

@@ -60,7 +60,7 @@ __device__ __forceinline__ void w4_store(const W4Args& a, int m, int n, const f3
 
 // ---- the bf16 form.  A wave owns NT column tiles x MT row tiles and every NW-th k block.  x goes from L2 straight into the wave's own
 // LDS (no registers, no writes on the way; through registers 18.0 instead of 16.4 us at 8192 -> 8192, 40 rows), a ring of NS stages of two
-// fragments (64 k): NS - 1 of them are always under way, and the next block's weights (two blocks' weights: 16.8 us, and 9.9 for 9.4 at one row).  A
+// fragments (64 k; one at four row tiles): NS - 1 of them are always under way, and the next block's weights (two blocks' weights: 16.8 us, and 9.9 for 9.4 at one row).  A
 // load is 16 rows x 64 bytes, four lanes to a row (a row per lane, as the fragments have it, runs at a quarter of the rate), and lands as it
 // comes, lane after lane; the 16-byte pieces of a row are asked for in the order c ^ (row / 2 mod 4), so that a fragment's read (eight
 // rows of one piece at a time) meets no bank twice.  Partial sums of the waves meet in LDS, in wave order.
@@ -81,11 +81,20 @@ __device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[2][3]) {
                  : "v"(at), "n"(1 << 10), "n"(2 << 10), "n"(3 << 10), "n"(4 << 10), "n"(5 << 10) : "memory");
 }
 
+// (four row tiles: one fragment)
+__device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[1][4]) {
+    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%5\n\tds_read_b128 %2, %4 offset:%6\n\tds_read_b128 %3, %4 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[0][2]), "=&v"(x[0][3]) : "v"(at), "n"(1 << 10), "n"(2 << 10), "n"(3 << 10) : "memory");
+}
+
 template <int G, int NT, int MT, int NW>
 __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
     constexpr int GPB = 128 / G, FPG = G / 32;                           // groups per k block, fragments per group
-    constexpr int NS = MT == 3 ? 3 : 4, STAGE = 2 * MT * 1024;           // bytes of a stage
-    constexpr int AHEAD = (NS - 1) * 2 * MT + NT * (1 + 2 * GPB);        // loads that may be under way while a stage is multiplied: the next ones, the next weights
+    constexpr int SF = MT == 4 ? 1 : 2, STEPS = 4 / SF;                  // fragments per stage, stages per block
+    constexpr int NS = MT == 3 ? 3 : 4, STAGE = SF * MT * 1024;          // bytes of a stage
+    // Loads younger than a stage's own, which may be under way while it is multiplied: NS - 1 stages, and the next block's weights (asked for
+    // with a block's first stage: the fourth of four stages is younger than they are)
+    constexpr int AHEAD = (NS - 1) * SF * MT, WEIGHTS = NT * (1 + 2 * GPB);
     const int nt0 = blockIdx.x * NT, m0 = blockIdx.y * 16 * MT, tiles = (a.N + 15) >> 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
     __shared__ f32x4 lds[NW * NS * STAGE / 16];                          // x of the waves, then their partial sums
@@ -118,13 +127,13 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
             }
         }
     };
-    // Stage i of this wave: half of block wave + NW (i / 2).  Behind the last block nothing moves; behind K (scales 0 there) the last
+    // Stage i of this wave: a half (quarter) of block wave + NW (i / STEPS).  Behind the last block nothing moves; behind K (scales 0 there) the last
     // fragment once more, which is a number wherever the row is.
     auto load_x = [&](int i, int slot) {
-        const int kb = wave + NW * (i >> 1);
+        const int kb = wave + NW * (i / STEPS);
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-            const int k = min(kb * 128 + (i & 1) * 64 + f * 32, a.K - 32);
+        for (int f = 0; f < SF; ++f) {
+            const int k = min(kb * 128 + (i % STEPS * SF + f) * 32, a.K - 32);
 #pragma unroll
             for (int t = 0; t < MT; ++t)
                 buf_load16_lds(xb, xl + slot * STAGE + (f * MT + t) * 1024, kb < a.KB ? xo[t] + k * 2 : BUF_OFF);
@@ -135,12 +144,12 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int t = 0; t < MT; ++t) acc[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto use = [&](const Stage& st, int half, int slot) {
-        bf16x8 x[2][MT];
+    auto use = [&](const Stage& st, int part, int slot) {
+        bf16x8 x[SF][MT];
         w4_read(xr + slot * STAGE, x);
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-            const int j = half * 2 + f, g = j / FPG;
+        for (int f = 0; f < SF; ++f) {
+            const int j = part * SF + f, g = j / FPG;
             const bf16 one = (bf16)1.0f;
             const bf16x8 ones = bf16x8{one, one, one, one, one, one, one, one};
             const f32x4 none = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -170,12 +179,18 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
         Stage A;
         if (wave < a.KB) {
             load_w(A, wave);
-            load_x(0, 0);
-            load_x(1, 1);
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * MT) : "memory");
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) load_x(i, i);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STEPS - 1) * SF * MT) : "memory");
             use(A, 0, 0);
+            if constexpr (STEPS == 4) {
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * SF * MT) : "memory");
+                use(A, 1, 1);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(SF * MT) : "memory");
+                use(A, 2, 2);
+            }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            use(A, 1, 1);
+            use(A, STEPS - 1, STEPS - 1);
         }
     } else {
         Stage A, B;
@@ -183,11 +198,12 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
 #pragma unroll
         for (int i = 0; i < NS - 1; ++i) load_x(i, i);
         int slot = 0, i = 0;
-        auto step = [&](const Stage& st, int half, bool on) {            // asks for stage i + NS - 1, multiplies stage i
+        auto step = [&](const Stage& st, int part, bool on) {            // asks for stage i + NS - 1, multiplies stage i
             load_x(i + NS - 1, slot == 0 ? NS - 1 : slot - 1);
             if (on) {
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(AHEAD) : "memory");
-                use(st, half, slot);
+                if (part == 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(AHEAD) : "memory");
+                else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(AHEAD + WEIGHTS) : "memory");
+                use(st, part, slot);
             }
             slot = slot == NS - 1 ? 0 : slot + 1;
             ++i;
@@ -196,11 +212,11 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
         // waits for those that are)
         for (int kb = wave; kb < a.KB; kb += 2 * NW) {
             load_w(B, kb + NW);
-            step(A, 0, true);
-            step(A, 1, true);
+#pragma unroll
+            for (int p = 0; p < STEPS; ++p) step(A, p, true);
             load_w(A, kb + 2 * NW);
-            step(B, 0, kb + NW < a.KB);
-            step(B, 1, kb + NW < a.KB);
+#pragma unroll
+            for (int p = 0; p < STEPS; ++p) step(B, p, kb + NW < a.KB);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                 // nothing more lands in LDS
     }
@@ -414,7 +430,8 @@ static void w4_launch_row(const W4Args& a, hipStream_t s) {
 }
 
 // Row tiles per workgroup: the fewest (more workgroups) that keep the launch within one workgroup per CU, else equal blocks of up to `most`
-// (8192 -> 8192, 32 rows as one block of two 13.4 us, as two of one 2 x 9.4; 40 rows on 1024 -> 1024 as three of one 3.1).
+// (8192 -> 8192, 32 rows as one block of two 13.4 us, as two of one 2 x 9.4; 64 rows as one of four 23.5, as two of two 24.9, and on
+// 1024 -> 8192 5.9 / 7.1; 40 rows on 1024 -> 1024 as three of one 3.1).
 static int w4_row_tiles(int M, int gx, int most) {
     for (int mt = 1; mt < most; ++mt)
         if ((long)gx * ceil_div(M, 16 * mt) <= 256) return mt;
@@ -422,11 +439,12 @@ static int w4_row_tiles(int M, int gx, int most) {
 }
 template <int G, int NT>
 static void w4_launch_bf16(const W4Args& a, hipStream_t s) {
-    const int gx = ceil_div(ceil_div(a.N, 16), NT), mt = w4_row_tiles(a.M, gx, 3);
+    const int gx = ceil_div(ceil_div(a.N, 16), NT), mt = w4_row_tiles(a.M, gx, 4);
     const dim3 grid(gx, ceil_div(a.M, 16 * mt));
     if (mt == 1) linear_w4_kernel<G, NT, 1, 8><<<grid, 512, 0, s>>>(a);
     else if (mt == 2) linear_w4_kernel<G, NT, 2, 8><<<grid, 512, 0, s>>>(a);
-    else linear_w4_kernel<G, NT, 3, 8><<<grid, 512, 0, s>>>(a);
+    else if (mt == 3) linear_w4_kernel<G, NT, 3, 8><<<grid, 512, 0, s>>>(a);
+    else linear_w4_kernel<G, NT, 4, 8><<<grid, 512, 0, s>>>(a);
 }
 template <int G>
 static void w4_launch(const W4Args& a, int dtype, hipStream_t s) {
