@@ -81,17 +81,18 @@ __device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[2][3]) {
                  : "v"(at), "n"(1 << 10), "n"(2 << 10), "n"(3 << 10), "n"(4 << 10), "n"(5 << 10) : "memory");
 }
 
-// (four row tiles: one fragment)
-__device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[1][4]) {
-    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%5\n\tds_read_b128 %2, %4 offset:%6\n\tds_read_b128 %3, %4 offset:%7\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[0][2]), "=&v"(x[0][3]) : "v"(at), "n"(1 << 10), "n"(2 << 10), "n"(3 << 10) : "memory");
+__device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[2][4]) {
+    asm volatile("ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:%9\n\tds_read_b128 %2, %8 offset:%10\n\tds_read_b128 %3, %8 offset:%11\n\t"
+                 "ds_read_b128 %4, %8 offset:%12\n\tds_read_b128 %5, %8 offset:%13\n\tds_read_b128 %6, %8 offset:%14\n\tds_read_b128 %7, %8 offset:%15\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[0][2]), "=&v"(x[0][3]), "=&v"(x[1][0]), "=&v"(x[1][1]), "=&v"(x[1][2]), "=&v"(x[1][3])
+                 : "v"(at), "n"(1 << 10), "n"(2 << 10), "n"(3 << 10), "n"(4 << 10), "n"(5 << 10), "n"(6 << 10), "n"(7 << 10) : "memory");
 }
 
 template <int G, int NT, int MT, int NW>
 __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
     constexpr int GPB = 128 / G, FPG = G / 32;                           // groups per k block, fragments per group
-    constexpr int SF = MT == 4 ? 1 : 2, STEPS = 4 / SF;                  // fragments per stage, stages per block
-    constexpr int NS = MT == 3 ? 3 : 4, STAGE = SF * MT * 1024;          // bytes of a stage
+    constexpr int SF = 2, STEPS = 4 / SF;                  // fragments per stage, stages per block
+    constexpr int NS = MT == 4 ? 2 : MT == 3 ? 3 : 4, STAGE = SF * MT * 1024;          // bytes of a stage
     // Loads younger than a stage's own, which may be under way while it is multiplied: NS - 1 stages, and the next block's weights (asked for
     // with a block's first stage: the fourth of four stages is younger than they are)
     constexpr int AHEAD = (NS - 1) * SF * MT, WEIGHTS = NT * (1 + 2 * GPB);
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
         auto step = [&](const Stage& st, int part, bool on) {            // asks for stage i + NS - 1, multiplies stage i
             load_x(i + NS - 1, slot == 0 ? NS - 1 : slot - 1);
             if (on) {
-                if (part == 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(AHEAD) : "memory");
+                if (part >= NS - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(AHEAD) : "memory");
                 else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(AHEAD + WEIGHTS) : "memory");
                 use(st, part, slot);
             }
