@@ -59,20 +59,24 @@ __device__ __forceinline__ void w4_store(const W4Args& a, int m, int n, const f3
 }
 
 // ---- the bf16 form.  A wave owns NT column tiles x MT row tiles and every NW-th k block.  x goes from L2 straight into the wave's own
-// LDS (no registers, no writes on the way; through registers 18.0 instead of 16.4 us at 8192 -> 8192, 40 rows), a ring of NS stages of two
-// fragments (64 k; one at four row tiles): NS - 1 of them are always under way, and the next block's weights (two blocks' weights: 16.8 us, and 9.9 for 9.4 at one row).  A
+// LDS (no registers, no writes on the way; through registers 18.0 instead of 16.4 us at 8192 -> 8192, 40 rows), a ring of NS stages: a whole
+// k block up to two row tiles, half of one beyond (a fragment at a time, more of them under way: 18.2 us; every stage costs its reads' latency).
+// NS - 1 stages are always under way, and the next block's weights (two blocks' weights: 16.8 us, and 9.9 for 9.4 at one row).  A
 // load is 16 rows x 64 bytes, four lanes to a row (a row per lane, as the fragments have it, runs at a quarter of the rate), and lands as it
 // comes, lane after lane; the 16-byte pieces of a row are asked for in the order c ^ (row / 2 mod 4), so that a fragment's read (eight
 // rows of one piece at a time) meets no bank twice.  Partial sums of the waves meet in LDS, in wave order.
 template <int GPB, int NT> struct W4Stage { uint4 w[NT]; uint2 s[GPB][NT]; uint32_t z[GPB][NT]; };
 
-// the two fragments of a stage, MT row tiles each (the compiler would wait for every load into LDS first)
-__device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[2][1]) {
-    asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:1024\n\ts_waitcnt lgkmcnt(0)" : "=&v"(x[0][0]), "=&v"(x[1][0]) : "v"(at) : "memory");
-}
-__device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[2][2]) {
+// the fragments of a stage, MT row tiles each (the compiler would wait for every load into LDS first)
+__device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[4][1]) {
     asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%5\n\tds_read_b128 %2, %4 offset:%6\n\tds_read_b128 %3, %4 offset:%7\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1]) : "v"(at), "n"(1 << 10), "n"(2 << 10), "n"(3 << 10) : "memory");
+                 : "=&v"(x[0][0]), "=&v"(x[1][0]), "=&v"(x[2][0]), "=&v"(x[3][0]) : "v"(at), "n"(1 << 10), "n"(2 << 10), "n"(3 << 10) : "memory");
+}
+__device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[4][2]) {
+    asm volatile("ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:%9\n\tds_read_b128 %2, %8 offset:%10\n\tds_read_b128 %3, %8 offset:%11\n\t"
+                 "ds_read_b128 %4, %8 offset:%12\n\tds_read_b128 %5, %8 offset:%13\n\tds_read_b128 %6, %8 offset:%14\n\tds_read_b128 %7, %8 offset:%15\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1]), "=&v"(x[2][0]), "=&v"(x[2][1]), "=&v"(x[3][0]), "=&v"(x[3][1])
+                 : "v"(at), "n"(1 << 10), "n"(2 << 10), "n"(3 << 10), "n"(4 << 10), "n"(5 << 10), "n"(6 << 10), "n"(7 << 10) : "memory");
 }
 __device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[2][3]) {
     asm volatile("ds_read_b128 %0, %6\n\tds_read_b128 %1, %6 offset:%7\n\tds_read_b128 %2, %6 offset:%8\n\tds_read_b128 %3, %6 offset:%9\n\t"
@@ -91,10 +95,10 @@ __device__ __forceinline__ void w4_read(uint32_t at, bf16x8 (&x)[2][4]) {
 template <int G, int NT, int MT, int NW>
 __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
     constexpr int GPB = 128 / G, FPG = G / 32;                           // groups per k block, fragments per group
-    constexpr int SF = 2, STEPS = 4 / SF;                  // fragments per stage, stages per block
-    constexpr int NS = MT == 4 ? 2 : MT == 3 ? 3 : 4, STAGE = SF * MT * 1024;          // bytes of a stage
-    // Loads younger than a stage's own, which may be under way while it is multiplied: NS - 1 stages, and the next block's weights (asked for
-    // with a block's first stage: the fourth of four stages is younger than they are)
+    constexpr int SF = MT <= 2 ? 4 : 2, STEPS = 4 / SF;                  // fragments per stage, stages per block
+    constexpr int NS = MT == 3 ? 3 : 2, STAGE = SF * MT * 1024;          // bytes of a stage
+    // Loads younger than a stage's own, which may be under way while it is multiplied: NS - 1 stages, and the next block's weights unless
+    // the stage was asked for behind them (they are asked for with a block's first stage)
     constexpr int AHEAD = (NS - 1) * SF * MT, WEIGHTS = NT * (1 + 2 * GPB);
     const int nt0 = blockIdx.x * NT, m0 = blockIdx.y * 16 * MT, tiles = (a.N + 15) >> 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
@@ -128,7 +132,7 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
             }
         }
     };
-    // Stage i of this wave: a half (quarter) of block wave + NW (i / STEPS).  Behind the last block nothing moves; behind K (scales 0 there) the last
+    // Stage i of this wave: part i % STEPS of block wave + NW (i / STEPS).  Behind the last block nothing moves; behind K (scales 0 there) the last
     // fragment once more, which is a number wherever the row is.
     auto load_x = [&](int i, int slot) {
         const int kb = wave + NW * (i / STEPS);
@@ -182,13 +186,9 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_kernel(W4Args a) {
             load_w(A, wave);
 #pragma unroll
             for (int i = 0; i < STEPS; ++i) load_x(i, i);
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STEPS - 1) * SF * MT) : "memory");
-            use(A, 0, 0);
-            if constexpr (STEPS == 4) {
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * SF * MT) : "memory");
-                use(A, 1, 1);
+            if constexpr (STEPS == 2) {
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(SF * MT) : "memory");
-                use(A, 2, 2);
+                use(A, 0, 0);
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             use(A, STEPS - 1, STEPS - 1);
@@ -431,7 +431,7 @@ static void w4_launch_row(const W4Args& a, hipStream_t s) {
 }
 
 // Row tiles per workgroup: the fewest (more workgroups) that keep the launch within one workgroup per CU, else equal blocks of up to `most`
-// (8192 -> 8192, 32 rows as one block of two 13.4 us, as two of one 2 x 9.4; 64 rows as one of four 23.5, as two of two 24.9, and on
+// (8192 -> 8192, 32 rows as one block of two 13.4 us, as two of one 2 x 9.4; 64 rows as one of four 21.0, as two of two 24.9, and on
 // 1024 -> 8192 5.9 / 7.1; 40 rows on 1024 -> 1024 as three of one 3.1).
 static int w4_row_tiles(int M, int gx, int most) {
     for (int mt = 1; mt < most; ++mt)
