@@ -175,10 +175,11 @@ __device__ __forceinline__ void tree_clean_v(TreeTile<T>& t, int s, int r) {
 // waves per SIMD that the registers are held down to
 template <typename T> constexpr int tree_waves(int qb) { return qb == 4 ? 2 : qb == 2 ? 3 : sizeof(T) == 2 ? 4 : 3; }
 
-template <typename T, int QB, int NW>
+// WHOLE: a tile lies in one page (pages of 32 rows and more)
+template <typename T, int QB, int NW, bool WHOLE>
 __global__ __launch_bounds__(NW * 64, tree_waves<T>(QB)) void attn_tree_kernel(TreeArgs a) {
     typedef TreeTile<T> Tile;
-    constexpr int SUB = Tile::SUB, KT = 16 * SUB;
+    constexpr int SUB = Tile::SUB, KT = 16 * SUB, NP = WHOLE ? 1 : SUB, PK = KT / NP;       // pages of a tile, keys in each
     const int split = blockIdx.x, kvh = blockIdx.y % a.Hkv, qblk = blockIdx.y / a.Hkv, b = blockIdx.z;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int fr = lane & 15, fq = lane >> 4;
@@ -225,30 +226,36 @@ __global__ __launch_bounds__(NW * 64, tree_waves<T>(QB)) void attn_tree_kernel(T
     // moves no data, and the loads stay countable.
     const int mine = t0 + wave < t1 ? (t1 - t0 - wave + NW - 1) / NW : 0;
     const __amdgpu_buffer_rsrc_t tb = buf_rsrc(tab, a.width * 4);
-    auto page_of = [&](int i) {                                          // lane s (mod SUB): the page of sub-tile s of this wave's tile i
-        const int key = (t0 + wave + NW * i) * KT + (lane % SUB) * 16;
+    auto page_of = [&](int i) {                                          // lane s (mod NP): the page of part s of this wave's tile i
+        const int key = (t0 + wave + NW * i) * KT + (lane % NP) * PK;
         return (int)buf_load4(tb, i < mine && key < T_all ? (uint32_t)(key >> a.shift) * 4 : BUF_OFF);
     };
+    // (The scalar work of a tile counts: a descriptor per page and tensor; with one per 16 keys whatever the page 70.5 instead of 67.6 us for
+    // 1 x 130,001 keys, 64 nodes, and 28.4 / 26.2 for 32,768.)
     auto load = [&](Tile& t, int i, int pages) {
         t.live = 0;
         uint32_t ko = lane * 16, vo = (fq * 256 + fr * 4) * (int)sizeof(T);
         asm("" : "+v"(ko), "+v"(vo));                                    // (kept next to the loads: their constants go into the instructions, not registers)
 #pragma unroll
-        for (int s = 0; s < SUB; ++s) {
-            const int page = __builtin_amdgcn_readlane(pages, s), key = (t0 + wave + NW * i) * KT + s * 16;
-            const bool on = i < mine && key < T_all && page >= 0 && page < a.n_pages;
-            const uint64_t at = (uint64_t)(uint32_t)(on ? page : 0) * page_bytes + (uint32_t)((key & ((1 << a.shift) - 1)) * 64 * (int)sizeof(T));
-            const uint32_t bytes = on ? min(16, T_all - key) * 64 * (int)sizeof(T) : 0;      // rows behind the sequence read zeros
+        for (int s = 0; s < NP; ++s) {
+            const int page = __builtin_amdgcn_readlane(pages, s), key = (t0 + wave + NW * i) * KT + s * PK;
+            const bool on = i < mine && key < T_all && (uint32_t)page < (uint32_t)a.n_pages;
+            const uint64_t at = (uint64_t)(uint32_t)page * page_bytes + (uint32_t)((key & ((1 << a.shift) - 1)) * 64 * (int)sizeof(T));
+            const uint32_t bytes = on ? min(PK, T_all - key) * 64 * (int)sizeof(T) : 0;      // rows behind the sequence read zeros; 0: nothing is read, wherever `at` is
             const __amdgpu_buffer_rsrc_t k = buf_rsrc((const char*)kbase + at, bytes), v = buf_rsrc((const char*)vbase + at, bytes);
 #pragma unroll
-            for (int n = 0; n < 4 / SUB; ++n) t.k[s * (4 / SUB) + n] = buf_load16(k, ko + n * 1024);
+            for (int n = 0; n < 4 / NP; ++n) t.k[s * (4 / NP) + n] = buf_load16(k, ko + n * 1024);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t off = vo + r * 64 * (int)sizeof(T);
-                if constexpr (sizeof(T) == 2) t.v[s][r] = __builtin_bit_cast(typename Tile::vrow, buf_load8(v, off));
-                else t.v[s][r] = __builtin_bit_cast(typename Tile::vrow, buf_load16(v, off));
+            for (int n = 0; n < 4 * (SUB / NP); ++n) {
+                const uint32_t off = vo + (n / 4 * 16 + n % 4) * 64 * (int)sizeof(T);
+                typename Tile::vrow& row = t.v[s * (SUB / NP) + n / 4][n % 4];
+                if constexpr (sizeof(T) == 2) row = __builtin_bit_cast(typename Tile::vrow, buf_load8(v, off));
+                else row = __builtin_bit_cast(typename Tile::vrow, buf_load16(v, off));
             }
-            if (on) t.live |= 1u << s;
+            if (on) {
+                if constexpr (NP == SUB) t.live |= 1u << s;
+                else t.live = key + 16 < T_all ? 3u : 1u;
+            }
         }
     };
     TreeKeys<T> kf;
@@ -567,7 +574,11 @@ extern "C" size_t valle_attn_tree_workspace_bytes(int rows, int B, int max_nodes
 template <typename T>
 static void tree_launch(const TreeArgs& a, const TreeShape& t, int B, hipStream_t s) {
     const dim3 grid(a.nsplit, a.Hkv * t.blocks, B);
-    auto go = [&](auto qb, auto nw) { attn_tree_kernel<T, decltype(qb)::value, decltype(nw)::value><<<grid, decltype(nw)::value * 64, 0, s>>>(a); };
+    auto go = [&](auto qb, auto nw) {
+        constexpr int QB = decltype(qb)::value, NW = decltype(nw)::value;
+        if (sizeof(T) == 4 || a.shift >= 5) attn_tree_kernel<T, QB, NW, true><<<grid, NW * 64, 0, s>>>(a);
+        else if constexpr (sizeof(T) == 2) attn_tree_kernel<T, QB, NW, false><<<grid, NW * 64, 0, s>>>(a);
+    };
     const std::integral_constant<int, 1> one;
     const std::integral_constant<int, 2> two;
     const std::integral_constant<int, 4> four;
