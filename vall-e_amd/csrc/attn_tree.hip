@@ -6,12 +6,13 @@
 // LDS; V is loaded as 4 keys x 4 dims per lane and its 16-bit 4 x 4 blocks are turned in registers (8 v_perm per 16 keys).  The four or eight
 // waves of a workgroup split the keys, so do up to 64 workgroups (grid x) where requests and heads alone do not fill the chip; a second launch
 // joins their partial sums.  Inside the loop waves never wait for one another.
-// Bound: the K / V bytes (2 x T x Hkv x 64 x es) with few queries: 16 requests x 311 .. 761 keys x 16 heads, one token (35 MB) 7.1 us
-// = 5.0 TB/s; 32 x 1,800 .. 2,561 keys, 9 .. 26 nodes (290 MB) 46 us = 6.3 TB/s.  With 64 nodes x 4 grouped heads the bytes no longer
-// count (1 x 130,001 keys: 34 GFLOP in 63 us): without its exponentials that call takes 6 us less, without the P.V products 10, without
+// Bound: the K / V bytes (2 x T x Hkv x 64 x es) with few queries: 16 requests x 311 .. 761 keys x 16 heads, one token (35 MB) 6.7 us
+// = 5.3 TB/s; 32 x 1,800 .. 2,561 keys, 9 .. 26 nodes (290 MB) 45 us = 6.4 TB/s.  With 64 nodes x 4 grouped heads the bytes no longer
+// count (1 x 130,001 keys: 34 GFLOP in 60 us): without its exponentials that call takes 6 us less, without the P.V products 10, without
 // the loads 12, without K's way through LDS 2 -- two waves per SIMD (244 registers) cover each other's latencies in part.  Tried there and
 // not faster: products placed between the exponentials by scheduling groups, one block's P.V delayed under the next one's exponentials,
-// two loops (with and without masks: spills), query groups of a workgroup sharing tiles.
+// two loops (with and without masks: spills), query groups of a workgroup sharing tiles, pages of many tiles in one load, tiles requested into
+// L2 two ahead.
 #include "common.h"
 #include <algorithm>
 #include <type_traits>
