@@ -555,7 +555,8 @@ int valle_attn_tree(const void* q, int64_t q_row_stride, const void* kcache, con
 
 /* The accepted path of every tree becomes context, in all layers (layer_stride elements apart): cached row ctx_len[b] + path[b][j]
  * moves to ctx_len[b] + j, j < min(n_accept[b], max_path), max_path <= 64; a node number outside 0 .. 63 moves nothing.  All of a
- * request's rows are read before any is written.  len_out[b] = ctx_len[b] + n_accept[b] (not ctx_len itself; negative lengths stay).
+ * request's rows are read before any is written.  len_out[b] = ctx_len[b] + that many (not ctx_len itself;
+ * negative lengths stay).
  * n_accept must not pass the rows that were planned: pages behind n_blocks belong to others. */
 int valle_paged_kv_commit(void* kcache, void* vcache, int n_layers, int64_t layer_stride, const int32_t* block_table, int max_blocks,
                           int n_pages, int page_size, const int32_t* ctx_len, const int32_t* path, int max_path,

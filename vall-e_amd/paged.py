@@ -111,5 +111,5 @@ def kv_commit(k_cache, v_cache, block_table, ctx_len, path, n_accept):
     """The accepted nodes of every request's tree become context, in all layers: cached row ``ctx_len[b] + path[b][j]`` moves to
     ``ctx_len[b] + j`` for ``j < n_accept[b]`` (``path`` int32 [requests][up to 64], node numbers 0 .. 63; others stay where they
     are).  ``n_accept`` must not pass the rows that were planned.  Caches ``[n_layers][n_pages][kv_heads][page_size][64]``, changed in place.
-    Returns the new lengths ``ctx_len + n_accept`` (a negative ``ctx_len`` stays)."""
+    Returns the new lengths, ``ctx_len + n_accept`` with ``n_accept`` held to 0 .. the path's width (a negative ``ctx_len`` stays)."""
     return _S.kv_commit(k_cache, v_cache, block_table, ctx_len, path, n_accept)
