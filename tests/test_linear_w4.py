@@ -215,3 +215,33 @@ def test_linear_w4_long_and_wide(gpu_device, dtype, rows, n, k, group):
     pad = torch.full((rows, k + 8), float("nan"), dtype=dtype)
     pad[:, :k] = x
     check(m(d(pad)[:, :k]), *want, dtype)                                               # rows of a wider matrix: what lies between them is not theirs
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 3, 40])
+def test_linear_w4_c_entry_fp32_logits_and_wide_rows_of_c(gpu_device, dtype, rows):
+    """What the module does not offer: fp32 results with an fp32 bias (heads), and C wider than N, with a bias and a residual; nothing is
+    written between the rows."""
+    from vall_e_amd import _lib as L
+    n, k, group, ldc = 75, 352, 32, 90
+    q, s, z = make(n, k, group, True, dtype, 21)
+    x = torch.randn(rows, k, generator=torch.Generator().manual_seed(4)).to(dtype)
+    d = lambda t: t.to(gpu_device)
+    m = PL.HipLinear4.from_quantized(d(q), d(s), d(z), group_size=group)
+    xd, code, stream = d(x), L.dtype_code(dtype), L.stream_ptr(gpu_device)
+
+    def call(bias, resid, out, epi):
+        L.check(L.load().valle_linear_w4(L.ptr(xd), k, L.ptr(m.wq), L.ptr(m.scales), L.ptr(m.zeros), L.ptr(bias), None if resid is None else L.ptr(resid), L.ptr(out), rows, n, k,
+                                         group, ldc, epi, code, stream))
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(5))
+    out = torch.full((rows, ldc), 7.0, device=gpu_device)
+    call(d(bias), None, out, 3)
+    want, err = expect(x, q, s, z, group, bias=bias)
+    assert (out[:, n:] == 7).all() and ((out[:, :n].cpu().double() - want).abs() <= err + U32 * want.abs()).all()
+    bias, resid = bias.to(dtype), torch.randn(rows, ldc, generator=torch.Generator().manual_seed(6)).to(dtype)
+    out = torch.full((rows, ldc), 7.0, dtype=dtype, device=gpu_device)
+    bd, rd = d(bias), d(resid)
+    call(bd, rd, out, 1)
+    assert (out[:, n:] == 7).all()
+    check(out[:, :n], *expect(x, q, s, z, group, bias=bias, resid=resid[:, :n]), dtype)
