@@ -557,7 +557,14 @@ int valle_attn_tree(const void* q, int64_t q_row_stride, const void* kcache, con
  * moves to ctx_len[b] + j, j < min(n_accept[b], max_path), max_path <= 64; a node number outside 0 .. 63 moves nothing.  All of a
  * request's rows are read before any is written.  len_out[b] = ctx_len[b] + that many (not ctx_len itself;
  * negative lengths stay).
- * n_accept must not pass the rows that were planned: pages behind n_blocks belong to others. */
+ * _served takes what the plan said of the requests, so that nothing need be read back in between: status [B] (NULL: all 0): a request with another
+ * one accepts nothing and keeps its length; n_blocks [B] (NULL: max_blocks each): rows at and behind n_blocks[b] pages are absent -- not read, not written
+ * --, and a served request's new length does not pass them.  Without n_blocks every table entry up to max_blocks is followed: the caller
+ * answers for n_accept not passing the rows that were planned, also where a request was refused (entries behind n_blocks name pages of others). */
+int valle_paged_kv_commit_served(void* kcache, void* vcache, int n_layers, int64_t layer_stride, const int32_t* block_table, int max_blocks,
+                                 int n_pages, int page_size, const int32_t* ctx_len, const int32_t* n_blocks, const int32_t* status,
+                                 const int32_t* path, int max_path, const int32_t* n_accept, int32_t* len_out, int B, int Hkv, int Dh, int dtype,
+                                 void* stream);
 int valle_paged_kv_commit(void* kcache, void* vcache, int n_layers, int64_t layer_stride, const int32_t* block_table, int max_blocks,
                           int n_pages, int page_size, const int32_t* ctx_len, const int32_t* path, int max_path,
                           const int32_t* n_accept, int32_t* len_out, int B, int Hkv, int Dh, int dtype, void* stream);

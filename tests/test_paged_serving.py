@@ -744,6 +744,112 @@ def test_kv_commit_layer_slices_and_counts_out_of_range(gpu_device):
     assert torch.equal(kc, k0)
 
 
+def ref_commit(kc, vc, table, ctx, path, acc, page, n_blocks, status):
+    """The commit as a scheduler would write it, request after request: (k, v, new lengths)."""
+    out, lens = [c.clone() for c in (kc, vc)], []
+    for b, c in enumerate(ctx):
+        held, fine = (table.shape[1] if n_blocks is None else n_blocks[b]) * page, status is None or status[b] == 0
+        n = min(max(acc[b], 0), len(path[b])) if fine else 0
+        lens.append(c if c < 0 else min(c + n, held) if fine and n_blocks is not None else c + n)
+        for j in range(n if c >= 0 else 0):
+            s, d = c + int(path[b][j]), c + j
+            if 0 <= path[b][j] < 64 and s < held and d < held:
+                for new, old in zip(out, (kc, vc)):
+                    new[:, table[b, d // page], :, d % page] = old[:, table[b, s // page], :, s % page]
+    return out[0], out[1], lens
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_refused_request_leaves_the_pages_of_others(gpu_device, dtype):
+    """A step in which the pool runs dry in front of one request, its drafted nodes accepted all the same (nothing is read back in between): its
+    left-over table entry names page 0, another request's.  Every page but the served ones' rows stays bit for bit, its length too; a later plan
+    serves it."""
+    dev, page, layers, kv = gpu_device, 16, 2, 2
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    table = P.PageTable(3, 6, 7, page, 128, device=dev)
+    table.plan(i32([0, 0, 0]), i32([30, 40, 10]))
+    assert table.n_blocks.tolist() == [2, 3, 1] and table.free_count.item() == 1
+    length = i32([30, 40, 10])
+    kc, vc = randn((layers, 7, kv, page, 64), dtype, 1, dev), randn((layers, 7, kv, page, 64), dtype, 2, dev)
+    nodes = [3, 20, 5]                                          # 33 rows need the last page, 60 rows one that is not there, 15 none
+    table.plan(length, length + i32(nodes), parents=i32([-1, 0, 1] + [-1] * 20 + list(range(-1, 4)) + [0] * 100))
+    assert table.status.tolist() == [0, 1, 0] and table.n_blocks.tolist() == [3, 3, 1] and table.block_table[1, 3].item() == 0 and table.block_table[0, 0].item() == 0
+    rows = sum(nodes)
+    q, k, v = (randn((rows, heads, 64), dtype, 3 + heads, dev) for heads in (4, kv, kv))
+    for l in range(layers):
+        k0, v0 = kc[l].clone(), vc[l].clone()
+        t = P.rope_kv_paged(q, k, v, table.positions[:rows].contiguous(), rope_table(64).to(dev), table.slots[:rows].contiguous(), kc[l], vc[l])
+        for s in table.slots[:rows].tolist():
+            if s >= 0:
+                k0[s // page, :, s % page], v0[s // page, :, s % page] = kc[l, s // page, :, s % page], vc[l, s // page, :, s % page]
+        assert torch.equal(kc[l], k0) and torch.equal(vc[l], v0)
+        P.attn_tree(t, kc[l], vc[l], table.block_table, length, table.cu_rows, table.tree_mask[:rows].contiguous(), max_nodes=20)
+        assert torch.equal(kc[l], k0) and torch.equal(vc[l], v0)
+    path = [[0, 1, 2] + [0] * 17, list(range(6, 20)) + [0] * 6, [1, 2, 4] + [0] * 17]
+    acc = [3, 14, 3]
+    want = ref_commit(kc.cpu(), vc.cpu(), table.block_table.cpu().numpy(), length.tolist(), path, acc, page, table.n_blocks.tolist(), table.status.tolist())
+    out = P.kv_commit(kc, vc, table.block_table, length, i32(path), i32(acc), table.n_blocks, table.status)
+    assert out.tolist() == want[2] == [33, 40, 13]
+    assert torch.equal(kc.cpu(), want[0]) and torch.equal(vc.cpu(), want[1])
+    table.plan(out, i32([0, 41, 13]))                           # the first request ends: there is room again
+    assert table.status.tolist() == [0, 0, 0] and table.n_blocks.tolist() == [0, 3, 1]
+    table.plan(out, i32([0, 60, 13]))
+    assert table.status.tolist() == [0, 0, 0] and table.n_blocks.tolist() == [0, 4, 1]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 64])
+def test_kv_commit_inside_the_pages_held(gpu_device, dtype, page):
+    """Any status, any n_accept and path, left-over entries that name the pages of others (or nothing): only the rows of served requests
+    inside the pages they hold are read or written; both arguments alone and none of them too."""
+    dev, layers, kv, n = gpu_device, 2, 3, 24
+    rs = np.random.default_rng(page)
+    width = 192 // page
+    i32 = lambda v: torch.from_numpy(np.asarray(v, dtype=np.int32)).to(dev)
+    held = [int(rs.integers(0, width + 1)) for _ in range(n)]
+    ctx = [int(rs.integers(0, max(1, h * page))) if rs.random() < 0.9 else -2 for h in held]
+    ctx[0], held[0] = 100, 0                                    # an ended request
+    ctx[1], held[1] = 2 * page, 2                               # a full last page: its first new row would lie behind it
+    pool = sum(held) + 2
+    perm, at = rs.permutation(pool), 0
+    table = rs.integers(-3, pool + 3, (n, width)).astype(np.int32)
+    for b, h in enumerate(held):
+        table[b, :h] = perm[at:at + h]
+        at += h
+    kc, vc = randn((layers, pool, kv, page, 64), dtype, 1, dev), randn((layers, pool, kv, page, 64), dtype, 2, dev)
+    path = np.stack([rs.permutation(66)[:64] - 1 for _ in range(n)]).astype(np.int32)
+    acc = [int(rs.integers(-2, 70)) for _ in range(n)]
+    status = [int(rs.choice([0, 0, 0, 1, 2, 3])) for _ in range(n)]
+    status[0] = status[1] = 0
+    for nb, st in ((held, status), (held, None)):
+        want = ref_commit(kc.cpu(), vc.cpu(), table, ctx, path, acc, page, nb, st)
+        k, v = kc.clone(), vc.clone()
+        out = P.kv_commit(k, v, i32(table), i32(ctx), i32(path), i32(acc), i32(nb), None if st is None else i32(st))
+        assert out.tolist() == want[2] and want[2][0] == 0 and want[2][1] == 2 * page
+        assert torch.equal(k.cpu(), want[0]) and torch.equal(v.cpu(), want[1])
+    none = [0 if s == 0 else a for s, a in zip(status, acc)]     # status alone: the served ones accept nothing here
+    k, v = kc.clone(), vc.clone()
+    assert P.kv_commit(k, v, i32(table), i32(ctx), i32(path), i32(none), status=i32(status)).tolist() == ctx and torch.equal(k, kc) and torch.equal(v, vc)
+    for kw in (dict(n_blocks=i32(held[:-1])), dict(status=i32(status).long()), dict(n_blocks=i32(held).cpu()), dict(status=i32(status + [0]))):
+        with pytest.raises(ValueError):
+            P.kv_commit(k, v, i32(table), i32(ctx), i32(path), i32(acc), **kw)
+
+
+def test_commit_entry_for_served_requests_refuses_bad_arguments():
+    import ctypes as C
+    from vall_e_amd import _lib as L
+    lib, p, o = L.load(), C.c_void_p(4096), C.c_void_p(8192)
+
+    def call(ctx=p, n_blocks=p, status=p, out=o, B=2, layers=2):
+        return lib.valle_paged_kv_commit_served(p, p, layers, 8 * 16 * 2 * 64, p, 4, 8, 16, ctx, n_blocks, status, p, 4, p, out, B, 2, 64, 1, None)
+    for kw in (dict(ctx=o), dict(n_blocks=o), dict(status=o), dict(ctx=None), dict(out=None), dict(layers=0), dict(B=-1)):
+        assert call(**kw) == -1, kw
+        assert b"valle_paged_kv_commit" in lib.valle_last_error()
+    assert call(B=0) == 0 and call(B=0, n_blocks=None, status=None) == 0
+
+
 @gpu
 def test_empty_calls(gpu_device):
     """No rows, no requests: nothing to do, nothing touched."""

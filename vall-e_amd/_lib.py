@@ -135,6 +135,8 @@ SIGNATURES = {
     "valle_attn_tree_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "valle_attn_tree": (c_int, [c_void_p, C.c_int64, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                 C.c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "valle_paged_kv_commit_served": (c_int, [c_void_p, c_void_p, c_int, C.c_int64, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                             c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
     "valle_paged_kv_commit": (c_int, [c_void_p, c_void_p, c_int, C.c_int64, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
                                       c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
     "valle_linear_w4": (c_int, [c_void_p, C.c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,

@@ -230,10 +230,10 @@ PyObject* attn_tree(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     CATCH
 }
 
-// (k_cache, v_cache, block_table, ctx_len, path, n_accept) -> new lengths
+// (k_cache, v_cache, block_table, ctx_len, path, n_accept, n_blocks | None, status | None) -> new lengths
 PyObject* kv_commit(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     TRY
-    ARGS(6);
+    ARGS(8);
     const at::Tensor &kc = tensor(a[0], "k_cache"), &vc = tensor(a[1], "v_cache"), &tab = tensor(a[2], "block_table"), &path = tensor(a[4], "path");
     const int dev = gpu_of(kc, "kv_commit"), dt = dtype_of(kc);
     pools(kc, vc, dev, kc.scalar_type(), true);
@@ -242,12 +242,14 @@ PyObject* kv_commit(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const int64_t B = tab.size(0), width = tab.size(1), wide = path.size(1);
     const int32_t *tp = ints(tab, "block_table", dev, {B, width}), *ctx = ints(tensor(a[3], "ctx_len"), "ctx_len", dev, {B});
     const int32_t *pp = ints(path, "path", dev, {B, wide}), *acc = ints(tensor(a[5], "n_accept"), "n_accept", dev, {B});
+    const at::Tensor *nb = maybe(a[6], "n_blocks"), *st = maybe(a[7], "status");
+    const int32_t *nbp = nb ? ints(*nb, "n_blocks", dev, {B}) : nullptr, *sp = st ? ints(*st, "status", dev, {B}) : nullptr;
     const at::Tensor out = fresh({B}, at::kInt, dev);
     if (B) {
         NEED(B <= INT32_MAX && width <= INT32_MAX && kc.size(0) <= INT32_MAX && kc.size(1) <= INT32_MAX, "kv_commit: sizes beyond 2^31");
         launch(dev, [&](void* s) {
-            return valle_paged_kv_commit(kc.data_ptr(), vc.data_ptr(), kc.size(0), kc.stride(0), tp, width, kc.size(1), kc.size(3), ctx, pp, wide, acc,
-                                         static_cast<int32_t*>(out.data_ptr()), B, kc.size(2), HEAD, dt, s);
+            return valle_paged_kv_commit_served(kc.data_ptr(), vc.data_ptr(), kc.size(0), kc.stride(0), tp, width, kc.size(1), kc.size(3), ctx, nbp, sp, pp, wide, acc,
+                                                static_cast<int32_t*>(out.data_ptr()), B, kc.size(2), HEAD, dt, s);
         });
     }
     return THPVariable_Wrap(out);

@@ -2,7 +2,8 @@
 // [n_pages][Hkv][page_size][64], a head's keys in one page contiguous as in the slot cache of valle_rope_kv.
 //   valle_page_plan          block tables, slot map, positions and tree masks from the requests' lengths
 //   valle_rope_kv_paged      RoPE on q and k rows, k and v into the pages the slot map names
-//   valle_paged_kv_commit    the accepted path of a draft tree to the end of the context, all layers
+//   valle_paged_kv_commit    the accepted path of a draft tree to the end of the context, all layers; valle_paged_kv_commit_served:
+//                            for the requests that the plan served, inside the pages they hold
 // The reference has no counterpart: it recomputes the whole sequence per step (models/base.py:521, use_cache=False).
 #include "common.h"
 
@@ -479,12 +480,14 @@ extern "C" int valle_rope_kv_paged(const void* q, int64_t q_row_stride, const vo
 
 // ------------------------------------------------------------------------------------ commit of an accepted path
 // cache[layer][ctx + j] = cache[layer][ctx + path[j]], j < n_accept.  Source and destination ranges overlap: a workgroup reads
-// every row it moves of one (request, head, layer) into registers, meets at a barrier, and writes.  Three dependent round trips (path,
+// every row it moves of one (request, head, layer) into registers, meets at a barrier, and writes.  With the plan's status and page counts a
+// request that was not served moves nothing, and no table entry at or behind its page count is followed: such entries are left over
+// and name pages of others.  Three dependent round trips (path,
 // table, row) bound it while the rows are few: one request, 12 layers, 3 rows 2.4 us; 16 requests, 5 rows 4.1; 48 requests, 26 rows (123 MB) 19 us
 // = 6.5 TB/s.
 struct CommitArgs {
     void *kc, *vc;
-    const int32_t *table, *ctx, *path, *n_accept;
+    const int32_t *table, *ctx, *n_blocks, *status, *path, *n_accept;      // n_blocks, status: may be NULL (all entries hold, all were served)
     int32_t* len_out;
     long layer_stride;                  // elements
     int width, max_path, n_pages, shift, Hkv;
@@ -496,13 +499,17 @@ __global__ __launch_bounds__(256) void kv_commit_kernel(CommitArgs a) {
     const int h = blockIdx.x, b = blockIdx.y;
     const long layer = blockIdx.z;
     const int ctx = a.ctx[b];
-    const int n = min(max(a.n_accept[b], 0), a.max_path);
-    if (h == 0 && layer == 0 && threadIdx.x == 0) a.len_out[b] = ctx < 0 ? ctx : ctx + n;
+    const bool served = !a.status || a.status[b] == 0;
+    const long cap = (long)(a.n_blocks ? min(max(a.n_blocks[b], 0), a.width) : a.width) << a.shift;
+    const int n = served ? min(max(a.n_accept[b], 0), a.max_path) : 0;
+    if (h == 0 && layer == 0 && threadIdx.x == 0) {
+        const long len = min((long)ctx + n, a.n_blocks && served ? cap : (long)INT32_MAX);
+        a.len_out[b] = ctx < 0 ? ctx : (int)len;
+    }
     if (ctx < 0 || n == 0) return;
     const int c = threadIdx.x % CH, isv = (threadIdx.x / CH) & 1, t0 = threadIdx.x / (2 * CH);
     T* cache = (T*)(isv ? a.vc : a.kc) + layer * a.layer_stride;
     const int32_t* tab = a.table + (long)b * a.width;
-    const long cap = (long)a.width << a.shift;
     auto place = [&](long p) -> long {                                  // element offset of cached row p, -1: not in the cache
         if (p >= cap) return -1;
         const int page = tab[p >> a.shift];
@@ -533,11 +540,13 @@ __global__ __launch_bounds__(256) void kv_commit_kernel(CommitArgs a) {
         if (dst[i] >= 0) *reinterpret_cast<uint4*>(cache + dst[i]) = x[i];
 }
 
-extern "C" int valle_paged_kv_commit(void* kcache, void* vcache, int n_layers, int64_t layer_stride, const int32_t* block_table, int max_blocks,
-                                     int n_pages, int page_size, const int32_t* ctx_len, const int32_t* path, int max_path,
-                                     const int32_t* n_accept, int32_t* len_out, int B, int Hkv, int Dh, int dtype, void* stream) {
+extern "C" int valle_paged_kv_commit_served(void* kcache, void* vcache, int n_layers, int64_t layer_stride, const int32_t* block_table, int max_blocks,
+                                            int n_pages, int page_size, const int32_t* ctx_len, const int32_t* n_blocks, const int32_t* status,
+                                            const int32_t* path, int max_path, const int32_t* n_accept, int32_t* len_out, int B, int Hkv, int Dh,
+                                            int dtype, void* stream) {
     VALLE_REQUIRE(kcache && vcache && block_table && ctx_len && path && n_accept && len_out, VALLE_E_ARG, "valle_paged_kv_commit: null pointer");
-    VALLE_REQUIRE(len_out != ctx_len, VALLE_E_ARG, "valle_paged_kv_commit: len_out must not be ctx_len (every workgroup reads the lengths)");
+    VALLE_REQUIRE(len_out != ctx_len && len_out != n_blocks && len_out != status, VALLE_E_ARG,
+                  "valle_paged_kv_commit: len_out must not be ctx_len, n_blocks or status (every workgroup reads them)");
     VALLE_REQUIRE(dtype == VALLE_BF16 || dtype == VALLE_F32, VALLE_E_ARG, "valle_paged_kv_commit: unknown dtype %d", dtype);
     VALLE_REQUIRE(Dh == 64, VALLE_E_UNSUPPORTED, "valle_paged_kv_commit: head_dim %d (64 is built)", Dh);
     VALLE_REQUIRE(B >= 0 && B <= 65535 && n_layers > 0 && n_layers <= 65535 && Hkv > 0 && max_blocks > 0, VALLE_E_ARG,
@@ -549,11 +558,18 @@ extern "C" int valle_paged_kv_commit(void* kcache, void* vcache, int n_layers, i
     VALLE_REQUIRE(n_layers == 1 || layer_stride >= ((int64_t)n_pages << shift) * Hkv * 64, VALLE_E_ARG, "valle_paged_kv_commit: layers overlap");
     VALLE_REQUIRE((((uintptr_t)kcache | (uintptr_t)vcache) & 15) == 0 && layer_stride % 8 == 0, VALLE_E_ARG, "valle_paged_kv_commit: caches must be 16-byte aligned");
     if (B == 0) return VALLE_OK;
-    CommitArgs a{kcache, vcache, block_table, ctx_len, path, n_accept, len_out, layer_stride, max_blocks, max_path, n_pages, shift, Hkv};
+    CommitArgs a{kcache, vcache, block_table, ctx_len, n_blocks, status, path, n_accept, len_out, layer_stride, max_blocks, max_path, n_pages, shift, Hkv};
     dim3 grid(Hkv, B, n_layers);
     hipStream_t s = (hipStream_t)stream;
     if (dtype == VALLE_BF16) kv_commit_kernel<bf16><<<grid, 256, 0, s>>>(a);
     else kv_commit_kernel<float><<<grid, 256, 0, s>>>(a);
     VALLE_LAUNCH_CHECK();
     return VALLE_OK;
+}
+
+extern "C" int valle_paged_kv_commit(void* kcache, void* vcache, int n_layers, int64_t layer_stride, const int32_t* block_table, int max_blocks,
+                                     int n_pages, int page_size, const int32_t* ctx_len, const int32_t* path, int max_path,
+                                     const int32_t* n_accept, int32_t* len_out, int B, int Hkv, int Dh, int dtype, void* stream) {
+    return valle_paged_kv_commit_served(kcache, vcache, n_layers, layer_stride, block_table, max_blocks, n_pages, page_size, ctx_len, nullptr, nullptr, path,
+                                        max_path, n_accept, len_out, B, Hkv, Dh, dtype, stream);
 }

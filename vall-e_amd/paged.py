@@ -4,7 +4,7 @@ drafted tokens per request.  One step of a loop, per layer where it says so:
     table.plan(len_old, len_new, parents)                       # pages, slots, positions, tree masks -- on the device, no sync
     q = rope_kv_paged(q, k, v, table.positions, rope, table.slots, k_cache[l], v_cache[l])               # per layer
     o = attn_tree(q, k_cache[l], v_cache[l], table.block_table, len_old, table.cu_rows, table.tree_mask)    # per layer
-    len_old = kv_commit(k_cache, v_cache, table.block_table, len_old, path, n_accept)     # the accepted nodes become context
+    len_old = kv_commit(k_cache, v_cache, table.block_table, len_old, path, n_accept, table.n_blocks, table.status)   # accepted nodes become context
 
 Caches are ``[n_layers][n_pages][kv_heads][page_size][64]`` (``kv_cache``), head_dim 64, bf16 or fp32, q and k heads
 pair-interleaved as the model's packed weights are (a rotation mixes elements 2i and 2i + 1).  The reference has no counterpart:
@@ -107,9 +107,14 @@ def attn_tree(q, k_cache, v_cache, block_table, ctx_len, cu_rows, tree_mask=None
                         HEAD_DIM ** -0.5 if softmax_scale is None else softmax_scale, out)
 
 
-def kv_commit(k_cache, v_cache, block_table, ctx_len, path, n_accept):
+def kv_commit(k_cache, v_cache, block_table, ctx_len, path, n_accept, n_blocks=None, status=None):
     """The accepted nodes of every request's tree become context, in all layers: cached row ``ctx_len[b] + path[b][j]`` moves to
     ``ctx_len[b] + j`` for ``j < n_accept[b]`` (``path`` int32 [requests][up to 64], node numbers 0 .. 63; others stay where they
-    are).  ``n_accept`` must not pass the rows that were planned.  Caches ``[n_layers][n_pages][kv_heads][page_size][64]``, changed in place.
-    Returns the new lengths, ``ctx_len + n_accept`` with ``n_accept`` held to 0 .. the path's width (a negative ``ctx_len`` stays)."""
-    return _S.kv_commit(k_cache, v_cache, block_table, ctx_len, path, n_accept)
+    are).  Caches ``[n_layers][n_pages][kv_heads][page_size][64]``, changed in place.  Returns the new lengths, ``ctx_len + n_accept`` with
+    ``n_accept`` held to 0 .. the path's width (a negative ``ctx_len`` stays).
+
+    ``n_blocks`` and ``status`` (int32 [requests], the table's after ``plan``; ``next_n_blocks`` after a plan that was not in place): a request
+    that was not served accepts nothing and keeps its length, whatever ``n_accept`` says; rows behind the pages a request holds are absent, and its
+    length does not pass them (an ended request's becomes 0; for requests that are cut short pass the shorter of both lengths as ``ctx_len``).  Without them ``n_accept`` must not pass the rows that were planned, and has to be 0 where
+    the plan refused the request: the table's entries behind ``n_blocks`` are left over and name pages of others."""
+    return _S.kv_commit(k_cache, v_cache, block_table, ctx_len, path, n_accept, n_blocks, status)
