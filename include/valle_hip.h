@@ -527,6 +527,12 @@ int valle_page_plan(const int32_t* len_old, const int32_t* len_new, int B, int p
                     const int32_t* n_blocks_in, int32_t* n_blocks_out, int32_t* free_list, int n_pages,
                     const int32_t* free_count_in, int32_t* free_count_out, int32_t* status, int32_t* cu_rows,
                     int32_t* slots, int32_t* positions, int max_rows, const int32_t* parents, int64_t* tree_mask, int32_t* ticket, void* stream);
+/* The same, tree_mask [max_rows] written by every plan: without parents (NULL) it holds chains, bits 0 .. i for row i of a request (all of them from
+ * row 63 on) and 0 behind the last row, so that one valle_attn_tree call serves tables of both kinds. */
+int valle_page_plan_masked(const int32_t* len_old, const int32_t* len_new, int B, int page_size, int32_t* block_table, int max_blocks,
+                           const int32_t* n_blocks_in, int32_t* n_blocks_out, int32_t* free_list, int n_pages,
+                           const int32_t* free_count_in, int32_t* free_count_out, int32_t* status, int32_t* cu_rows,
+                           int32_t* slots, int32_t* positions, int max_rows, const int32_t* parents, int64_t* tree_mask, int32_t* ticket, void* stream);
 
 /* valle_rope_kv for pages: q [M][H][64], k, v [M][Hkv][64] (row strides in elements, rows 16-byte aligned), q and k rotated by
  * rope[positions[m]] ([rope_rows][32][2] fp32; a position outside takes the nearest row), q to q_out (q_out == q is allowed; both

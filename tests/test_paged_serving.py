@@ -354,6 +354,66 @@ def test_plan_there_and_back_keeps_every_page(gpu_device):
         assert nb == [max(blocks(c, page), 0) for c in lens]
 
 
+@gpu
+@pytest.mark.parametrize("n,max_rows", [(1, 64), (5, 400), (64, 3000), (65, 3000), (512, 5000), (600, 3000), (600, 9000)])
+def test_plain_plan_behind_a_tree_plan(gpu_device, n, max_rows):
+    """One table, planned with trees and then without: no bit of the trees stays in tree_mask, which holds the chains that attn_tree takes for no
+    mask; the same where a captured plan with trees was replayed in between."""
+    rs = np.random.default_rng(n + max_rows)
+    dev, page = gpu_device, 16
+    t = P.PageTable(n, 12, n * 12, page, max_rows, device=dev)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    zero, trees = i32([0] * n), i32([min(4, max_rows // n)] * n)
+    par = i32([-1] * max_rows)                                  # stars: a node sees itself alone
+    t.plan(zero, trees, parents=par, in_place=False)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        t.plan(zero, trees, parents=par, in_place=False)
+    lo = [int(v) for v in rs.integers(0, 90, n)]
+    t.plan(zero, i32(lo))                                       # the contexts' pages
+    for new in ([int(rs.integers(0, 100 if n < 10 else 3)) for _ in lo], [1] * n, [0] * n):
+        graph.replay()
+        nodes, star = int(trees[0]) * n, 2 ** (torch.arange(max_rows) % int(trees[0]))
+        star[nodes:] = 0
+        assert torch.equal(t.tree_mask.cpu(), star)
+        t.plan(i32(lo), i32([a + b for a, b in zip(lo, new)]), in_place=False)
+        rows = [min(i, 63) for k in new for i in range(k)][:max_rows]
+        assert t.tree_mask.tolist() == [(1 << (i + 1)) - 1 if i < 63 else -1 for i in rows] + [0] * (max_rows - len(rows))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_plain_step_with_the_table_s_mask(gpu_device, dtype):
+    """A drafted step, then a plain one, both as the module's documentation writes them: tree_mask handed on whatever the plan was."""
+    dev, page = gpu_device, 16
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    t = P.PageTable(3, 8, 24, page, 128, device=dev)
+    kc, vc = randn((24, 2, page, 64), dtype, 1, dev), randn((24, 2, page, 64), dtype, 2, dev)
+    q = randn((128, 4, 64), dtype, 3, dev)
+    length = i32([20, 0, 47])
+    t.plan(i32([0, 0, 0]), length)
+    t.plan(length, i32([23, 9, 50]), parents=i32([-1] * 128))
+    drafted = P.attn_tree(q, kc, vc, t.block_table, length, t.cu_rows, t.tree_mask, 9)
+    length, new = i32([21, 1, 48]), i32([1, 3, 1])
+    t.plan(length, length + new)
+    got = P.attn_tree(q, kc, vc, t.block_table, length, t.cu_rows, t.tree_mask, 3)
+    want = P.attn_tree(q, kc, vc, t.block_table, length, t.cu_rows, None, 3)
+    assert torch.equal(got[:5], want[:5]) and not torch.equal(got[:5], drafted[:5])
+    check_attn(got[:5], (q[:5].cpu(), kc.cpu(), vc.cpu(), t.block_table.cpu().numpy(), length.tolist(), t.cu_rows.tolist(), None))
+
+
+def test_masked_plan_entry_refuses_bad_arguments():
+    import ctypes as C
+    from vall_e_amd import _lib as L
+    lib, p = L.load(), C.c_void_p(4096)
+
+    def plan(lo=p, B=2, page=16, max_rows=64, mask=p):
+        return lib.valle_page_plan_masked(lo, p, B, page, p, 4, p, p, p, 8, p, p, p, p, p, p, max_rows, None, mask, p, None)
+    for kw in (dict(mask=None), dict(lo=None), dict(B=0), dict(page=24), dict(max_rows=0)):
+        assert plan(**kw) == -1, kw
+        assert b"valle_page_plan" in lib.valle_last_error()
+
+
 # --------------------------------------------------------------------------------------- RoPE + write
 def randn(shape, dtype, seed, dev):
     return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(dev)

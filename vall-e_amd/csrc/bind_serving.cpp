@@ -153,7 +153,7 @@ PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const int32_t* lo = ints(tensor(a[0], "len_old"), "len_old", dev, {B});
     const int32_t* ln = ints(tensor(a[1], "len_new"), "len_new", dev, {B});
     const int32_t* pp = par ? ints(*par, "parents", dev, {rows}) : nullptr;
-    int64_t* mask = par ? ints<int64_t>(tensor(a[13], "tree_mask"), "tree_mask", dev, {rows}) : nullptr;
+    int64_t* mask = ints<int64_t>(tensor(a[13], "tree_mask"), "tree_mask", dev, {rows});
     int32_t* tp = ints(tab, "block_table", dev, {B, width});
     const int32_t *nb = ints(tensor(a[4], "n_blocks"), "n_blocks", dev, {B}), *fc = ints(tensor(a[7], "free_count"), "free_count", dev, {1});
     int32_t *nbo = ints(tensor(a[5], "n_blocks_out"), "n_blocks_out", dev, {B}), *fco = ints(tensor(a[8], "free_count_out"), "free_count_out", dev, {1});
@@ -161,7 +161,7 @@ PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     int32_t *sp = ints(slots, "slots", dev, {rows}), *ps = ints(tensor(a[12], "positions"), "positions", dev, {rows});
     int32_t* ticket = ints(tensor(a[14], "ticket"), "ticket", dev, {1});
     const int page = whole(a[15], "page_size");
-    launch(dev, [&](void* s) { return valle_page_plan(lo, ln, B, page, tp, width, nb, nbo, flp, pages, fc, fco, st, cu, sp, ps, rows, pp, mask, ticket, s); });
+    launch(dev, [&](void* s) { return valle_page_plan_masked(lo, ln, B, page, tp, width, nb, nbo, flp, pages, fc, fco, st, cu, sp, ps, rows, pp, mask, ticket, s); });
     Py_RETURN_NONE;
     CATCH
 }

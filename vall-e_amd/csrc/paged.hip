@@ -20,7 +20,7 @@ struct PlanArgs {
     int32_t* free_list;
     const int32_t* fc_in; int32_t* fc_out;
     int32_t *status, *cu, *slots, *pos;
-    const int32_t* parents; int64_t* mask;
+    const int32_t* parents; int64_t* mask;                    // parents NULL: plain rows, chains; mask NULL: none is written
     int32_t* ticket;
     int B, width, n_pages, shift, max_rows;
 };
@@ -66,13 +66,20 @@ __device__ __forceinline__ int plan_slot(const PlanArgs& a, int b, int p, bool s
     const int page = a.table[(size_t)b * a.width + blk];
     return page >= 0 && page < a.n_pages ? (page << a.shift) + (p & ((1 << a.shift) - 1)) : -1;
 }
+// the mask of row i of a chain: itself and the rows in front of it (from row 63 on a word holds no more)
+__device__ __forceinline__ int64_t plan_chain(int i) { return i < 63 ? (int64_t)((2ull << i) - 1) : -1; }
 // plain rows: row r belongs to the request whose end lies behind it; rows behind the last request are padding (slot -1)
 __device__ __forceinline__ void plan_row(const PlanArgs& a, const int* ends, const int* stat, int r) {
-    if (r >= ends[a.B - 1]) { a.slots[r] = -1; a.pos[r] = 0; return; }
-    const int b = plan_find(ends, a.B, r);
-    const int p = a.len_old[b] + r - (b ? ends[b - 1] : 0);
-    a.slots[r] = plan_slot(a, b, p, stat[b] == 0);
-    a.pos[r] = p;
+    int slot = -1, p = 0;
+    int64_t m = 0;
+    if (r < ends[a.B - 1]) {
+        const int b = plan_find(ends, a.B, r), i = r - (b ? ends[b - 1] : 0);
+        p = a.len_old[b] + i;
+        slot = plan_slot(a, b, p, stat[b] == 0);
+        m = plan_chain(i);
+    }
+    a.slots[r] = slot; a.pos[r] = p;
+    if (a.mask) a.mask[r] = m;
 }
 // tree rows of one request: lane i = node i, its slot given.  Ancestor bits and depths by pointer doubling (6 rounds cover 64 levels).
 __device__ __forceinline__ void plan_tree(const PlanArgs& a, int len_old, int start, int n, int slot, int lane) {
@@ -216,13 +223,15 @@ __global__ __launch_bounds__(1024) void page_plan_wave_kernel(PlanArgs a) {
     }
     for (long r = (a.parents ? all : 0) + (long)blockIdx.x * 1024 + threadIdx.x; r < a.max_rows; r += gridDim.x * 1024) {
         int slot = -1, pos = 0;
+        int64_t m = 0;
         if (r < all) {
-            const int b = plan_find(s_end, a.B, (int)r);
-            pos = s_lo[b] + (int)r - (b ? s_end[b - 1] : 0);
+            const int b = plan_find(s_end, a.B, (int)r), i = (int)r - (b ? s_end[b - 1] : 0);
+            pos = s_lo[b] + i;
             slot = slot_of(b, pos);
+            m = plan_chain(i);
         }
         a.slots[r] = slot; a.pos[r] = pos;
-        if (a.parents) a.mask[r] = 0;
+        if (a.mask) a.mask[r] = m;
     }
     if (wave == 0 && (gridDim.x == 1 || __builtin_amdgcn_readfirstlane(turn) == (int)gridDim.x - 1)) {
 #pragma unroll
@@ -352,10 +361,10 @@ static int page_shift(int page_size) {
     return -1;
 }
 
-extern "C" int valle_page_plan(const int32_t* len_old, const int32_t* len_new, int B, int page_size, int32_t* block_table, int max_blocks,
-                               const int32_t* n_blocks_in, int32_t* n_blocks_out, int32_t* free_list, int n_pages,
-                               const int32_t* free_count_in, int32_t* free_count_out, int32_t* status, int32_t* cu_rows,
-                               int32_t* slots, int32_t* positions, int max_rows, const int32_t* parents, int64_t* tree_mask, int32_t* ticket, void* stream) {
+static int page_plan(const int32_t* len_old, const int32_t* len_new, int B, int page_size, int32_t* block_table, int max_blocks,
+                     const int32_t* n_blocks_in, int32_t* n_blocks_out, int32_t* free_list, int n_pages,
+                     const int32_t* free_count_in, int32_t* free_count_out, int32_t* status, int32_t* cu_rows,
+                     int32_t* slots, int32_t* positions, int max_rows, const int32_t* parents, int64_t* tree_mask, int32_t* ticket, void* stream) {
     VALLE_REQUIRE(len_old && len_new && block_table && n_blocks_in && n_blocks_out && free_list && free_count_in && free_count_out && status && cu_rows &&
                   slots && positions && ticket, VALLE_E_ARG, "valle_page_plan: null pointer");
     VALLE_REQUIRE(B > 0 && B <= PLAN_MAX_B, VALLE_E_ARG, "valle_page_plan: %d requests (1 .. %d)", B, PLAN_MAX_B);
@@ -365,7 +374,6 @@ extern "C" int valle_page_plan(const int32_t* len_old, const int32_t* len_new, i
                   "valle_page_plan: max_blocks %d", max_blocks);
     VALLE_REQUIRE(n_pages > 0 && ((int64_t)n_pages << shift) <= INT32_MAX, VALLE_E_ARG, "valle_page_plan: n_pages %d", n_pages);
     VALLE_REQUIRE(max_rows > 0, VALLE_E_ARG, "valle_page_plan: max_rows %d", max_rows);
-    VALLE_REQUIRE((parents == nullptr) == (tree_mask == nullptr), VALLE_E_ARG, "valle_page_plan: parents and tree_mask go together");
     PlanArgs a{len_old, len_new, block_table, n_blocks_in, n_blocks_out, free_list, free_count_in, free_count_out, status, cu_rows, slots, positions,
                parents, tree_mask, ticket, B, max_blocks, n_pages, shift, max_rows};
     hipStream_t s = (hipStream_t)stream;
@@ -381,6 +389,24 @@ extern "C" int valle_page_plan(const int32_t* len_old, const int32_t* len_new, i
     }
     VALLE_LAUNCH_CHECK();
     return VALLE_OK;
+}
+
+extern "C" int valle_page_plan(const int32_t* len_old, const int32_t* len_new, int B, int page_size, int32_t* block_table, int max_blocks,
+                               const int32_t* n_blocks_in, int32_t* n_blocks_out, int32_t* free_list, int n_pages,
+                               const int32_t* free_count_in, int32_t* free_count_out, int32_t* status, int32_t* cu_rows,
+                               int32_t* slots, int32_t* positions, int max_rows, const int32_t* parents, int64_t* tree_mask, int32_t* ticket, void* stream) {
+    VALLE_REQUIRE((parents == nullptr) == (tree_mask == nullptr), VALLE_E_ARG, "valle_page_plan: parents and tree_mask go together");
+    return page_plan(len_old, len_new, B, page_size, block_table, max_blocks, n_blocks_in, n_blocks_out, free_list, n_pages, free_count_in, free_count_out, status,
+                     cu_rows, slots, positions, max_rows, parents, tree_mask, ticket, stream);
+}
+
+extern "C" int valle_page_plan_masked(const int32_t* len_old, const int32_t* len_new, int B, int page_size, int32_t* block_table, int max_blocks,
+                                      const int32_t* n_blocks_in, int32_t* n_blocks_out, int32_t* free_list, int n_pages,
+                                      const int32_t* free_count_in, int32_t* free_count_out, int32_t* status, int32_t* cu_rows,
+                                      int32_t* slots, int32_t* positions, int max_rows, const int32_t* parents, int64_t* tree_mask, int32_t* ticket, void* stream) {
+    VALLE_REQUIRE(tree_mask, VALLE_E_ARG, "valle_page_plan_masked: null pointer");
+    return page_plan(len_old, len_new, B, page_size, block_table, max_blocks, n_blocks_in, n_blocks_out, free_list, n_pages, free_count_in, free_count_out, status,
+                     cu_rows, slots, positions, max_rows, parents, tree_mask, ticket, stream);
 }
 
 // ------------------------------------------------------------------------------------ RoPE + write into pages

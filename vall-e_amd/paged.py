@@ -49,7 +49,7 @@ class PageTable:
     [max_requests], ``free_list`` [n_pages] (a stack of the first ``free_count[0]`` entries).
     Written by every ``plan``: ``cu_rows`` [max_requests + 1] (row offsets of the step's packed rows), ``slots`` / ``positions``
     [max_rows] (slot = page * page_size + offset; -1: padding row, or a request without pages), ``tree_mask`` [max_rows] int64
-    (with ``parents`` only), ``status`` [max_requests]: 0 served, 1 no pages left (it keeps what it had), 2 lengths out of range,
+    (plain rows: chains), ``status`` [max_requests]: 0 served, 1 no pages left (it keeps what it had), 2 lengths out of range,
     3 its rows lie behind ``max_rows``; what a step computes for rows of requests that were not served means nothing."""
 
     def __init__(self, max_requests, max_blocks, n_pages, page_size, max_rows, device="cuda"):
@@ -76,7 +76,7 @@ class PageTable:
         order until the pool is empty, and the rows ``len_old .. len_new`` get their slots.  ``parents`` (int32 [max_rows]): row r
         is a drafted node whose parent is node ``parents[r]`` of the same request, an earlier one (anything else: a child of the
         context); positions are then ``len_old`` + depth and ``tree_mask`` holds every node's ancestors and itself; at most 64
-        new rows per request.  ``in_place=False`` leaves ``n_blocks`` and ``free_count`` and writes ``next_n_blocks`` /
+        new rows per request.  Without them ``tree_mask`` holds what ``attn_tree`` takes for no mask: row i sees rows 0 .. i.  ``in_place=False`` leaves ``n_blocks`` and ``free_count`` and writes ``next_n_blocks`` /
         ``next_free_count`` (a plan that may be thrown away)."""
         if in_place:
             nb, fc = self.n_blocks, self.free_count
