@@ -245,3 +245,79 @@ def test_linear_w4_c_entry_fp32_logits_and_wide_rows_of_c(gpu_device, dtype, row
     call(bd, rd, out, 1)
     assert (out[:, n:] == 7).all()
     check(out[:, :n], *expect(x, q, s, z, group, bias=bias, resid=resid[:, :n]), dtype)
+
+
+# --------------------------------------------------------------------------------------- every bf16 form
+def form(rows, n):
+    """(column tiles, row tiles) per workgroup that the dispatch takes for bf16; test_dispatch_rule_is_the_one_restated_here holds it to the source."""
+    up = lambda a, b: -(-a // b)
+    nt = 2 if up(n, 32) * up(rows, 48) >= 256 else 1
+    gx = up(up(n, 16), nt)
+    for mt in (1, 2, 3):
+        if gx * up(rows, 16 * mt) <= 256:
+            return nt, mt
+    return nt, up(up(rows, up(rows, 64)), 16)
+
+
+# rows x columns of every form: with rows and columns that end inside a tile, and whole ones
+FORMS = {(1, 1): [(7, 4090), (16, 512)], (1, 2): [(23, 4090), (32, 4096)], (1, 3): [(37, 4090), (48, 4096)], (1, 4): [(57, 4060), (64, 4064)],
+         (2, 1): [(7, 8186), (16, 8192)], (2, 2): [(23, 8186), (32, 8192)], (2, 3): [(37, 8186), (48, 8192)], (2, 4): [(57, 8200), (64, 8192)]}
+# inputs by group: up to one k block of 128 per wave (eight waves), and several: an odd and an even number of blocks per wave, the last one whole and in part
+INPUTS = {32: [96, 992, 1184, 2176], 64: [192, 960, 1216, 2176], 128: [384, 1024, 1408, 2176]}
+
+
+def test_dispatch_rule_is_the_one_restated_here():
+    """A changed rule has to change form() and FORMS with it, so that no form drops out of the test below."""
+    from pathlib import Path
+    src = (Path(PL.__file__).parent / "csrc" / "linear_w4.hip").read_text()
+    for line in ("if ((long)ceil_div(a.N, 32) * ceil_div(a.M, 48) >= 256) w4_launch_bf16<G, 2>(a, s);",
+                 "const int gx = ceil_div(ceil_div(a.N, 16), NT), mt = w4_row_tiles(a.M, gx, 4);",
+                 "if ((long)gx * ceil_div(M, 16 * mt) <= 256) return mt;",
+                 "return ceil_div(ceil_div(M, ceil_div(M, 16 * most)), 16);",
+                 "if (mt == 1) linear_w4_kernel<G, NT, 1, 8><<<grid, 512, 0, s>>>(a);",
+                 "if (a.KB <= NW) {"):
+        assert line in src, line
+    for want, shapes in FORMS.items():
+        for rows, n in shapes:
+            assert form(rows, n) == want and n % 2 == 0
+    for group, ks in INPUTS.items():
+        assert all(k % group == 0 for k in ks) and sum(-(-k // 128) <= 8 for k in ks) == 2
+
+
+@gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("nt,mt", sorted(FORMS))
+@pytest.mark.parametrize("zeros", [False, True])
+def test_linear_w4_every_form(gpu_device, group, nt, mt, zeros):
+    """Every kernel that bf16 rows can reach -- group, column tiles, row tiles, one k block per wave or several -- with and without zero points and with
+    every epilogue; each has its own count of loads under way, so each runs three times on memory that the others have just used."""
+    from vall_e_amd import _lib as L
+    dtype, dev = torch.bfloat16, gpu_device
+    for i, k in enumerate(INPUTS[group]):
+        rows, n = FORMS[nt, mt][i % 2]
+        assert form(rows, n) == (nt, mt)
+        q, s, z = (None if t is None else t.to(dev) for t in make(n, k, group, zeros, dtype, k + nt + mt))
+        g = torch.Generator().manual_seed(k)
+        x = torch.randn(rows, k, generator=g).to(dtype).to(dev)
+        bias, resid = torch.randn(n, generator=g).to(dtype).to(dev), torch.randn(rows, n, generator=g).to(dtype).to(dev)
+        plain, biased = PL.HipLinear4.from_quantized(q, s, z, group_size=group), PL.HipLinear4.from_quantized(q, s, z, group_size=group, bias=bias)
+        y, err = expect(x, q, s, z, group)
+
+        def held(got, want, err, unit):
+            e = (got.double() - want).abs()
+            lim = err + unit * want.abs()
+            assert (e <= lim).all(), (rows, n, k, float((e - lim).max()), int((e > lim).sum()))
+        logits = torch.empty(rows, n, device=dev)
+        for _ in range(3):
+            held(plain(x), y, err, UNIT[dtype])
+            gate, up, eg, eu = y[:, 0::2], y[:, 1::2], err[:, 0::2], err[:, 1::2]
+            act = torch.nn.functional.gelu(gate)
+            held(plain(x, geglu=True), act * up, 1.13 * eg * (up.abs() + eu) + act.abs() * eu + 4e-7 * (gate * up).abs(), UNIT[dtype])
+            b = y + bias.double()
+            eb = err + 2 * U32 * (b.abs() + bias.double().abs())
+            held(biased(x), b, eb, UNIT[dtype])
+            r = b + resid.double()
+            held(biased(x, resid=resid), r, eb + 2 * U32 * (r.abs() + resid.double().abs()), UNIT[dtype])
+            L.check(L.load().valle_linear_w4(L.ptr(x), k, L.ptr(plain.wq), L.ptr(plain.scales), L.ptr(plain.zeros), None, None, L.ptr(logits), rows, n, k, group, n, L.EPI_F32OUT,
+                                             L.BF16, L.stream_ptr(dev)))
+            held(logits, y, err, U32)
