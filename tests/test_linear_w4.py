@@ -77,6 +77,21 @@ def test_quantize_w4_refuses_what_has_no_four_bits():
         PL.HipLinear4(64, 4).load_state_dict({"weight": torch.zeros(4, 128), "bias": torch.zeros(4)})
 
 
+def test_quantize_w4_refuses_a_range_without_a_finite_scale():
+    """Finite weights of both signs near the type's end: their range, and with it the scale, would be infinite."""
+    for dtype in (torch.float32, torch.bfloat16):
+        w = torch.zeros(2, 64, dtype=dtype)
+        w[1, 3], w[1, 9] = 3e38, -3e38
+        with pytest.raises(ValueError):
+            PL.quantize_w4(w, 64)
+        with pytest.raises(ValueError):
+            PL.HipLinear4(64, 2, dtype=dtype, bias=False).load_state_dict({"weight": w})
+        q, s, z = PL.quantize_w4(w, 64, symmetric=True)             # one sign's range is finite
+        assert torch.isfinite(s).all()
+        w[1, 9] = 0.0
+        assert torch.isfinite(PL.quantize_w4(w, 64)[1]).all()
+
+
 def test_packed_layout_holds_every_weight():
     """The documented layout, element by element."""
     n, k, group = 18, 160, 32

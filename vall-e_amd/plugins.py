@@ -89,7 +89,7 @@ class HipLinear(torch.nn.Module):
 def quantize_w4(weight, group_size=64, symmetric=False):
     """4-bit weights by groups of ``group_size`` along the input: ``(q, scales, zeros)`` with ``w ~ scales * (q - zeros)``, q uint8
     ``[out][in / 2]`` (two to a byte, the even input in the low nibble), scales ``[out][in / group]`` in the weight's type, zeros
-    uint8 of the same shape (None when symmetric: 8)."""
+    uint8 of the same shape (None when symmetric: 8).  Weights that are not finite, or whose range has no finite scale, raise ValueError."""
     n, k = weight.shape
     if k % group_size or not torch.isfinite(weight).all():
         raise ValueError(f"quantize_w4: finite weights and a group_size that divides {k} needed (got {group_size})")
@@ -101,6 +101,8 @@ def quantize_w4(weight, group_size=64, symmetric=False):
         lo, hi = w.amin(-1).clamp(max=0.0), w.amax(-1).clamp(min=0.0)
         s = ((hi - lo) / 15.0).to(weight.dtype).float()
         z = torch.where(s > 0, (-lo / s.clamp(min=torch.finfo(torch.float32).tiny)).round().clamp(0, 15), torch.zeros_like(s))
+    if not torch.isfinite(s).all():
+        raise ValueError("quantize_w4: a group's range passes its scale's type")
     d = torch.where(s > 0, s, torch.ones_like(s))
     q = (w / d[..., None] + z[..., None]).round().clamp(0, 15).to(torch.uint8).reshape(n, k)
     return q[:, 0::2] | (q[:, 1::2] << 4), s.to(weight.dtype), None if symmetric else z.to(torch.uint8)
