@@ -249,27 +249,25 @@ __device__ __forceinline__ int w4_place(int r, int c) { return c * 16 + (((r & 7
 
 // ---- the fp32 form: weights become (q - zero) * scale in fp32 (one rounding), the group structure ends there; an MFMA takes 4 inputs, the
 // k slots of a fragment are dealt so that a lane's 8 weights of a word meet its 8 values of x.  Two accumulators, for the dependent chain.
-template <int GPB, int MT> struct W4Stage32 { uint4 w; float s[GPB]; uint32_t z[GPB]; uint4 x[MT][8]; };
+template <int GPB> struct W4Stage32 { uint4 w; float s[GPB]; uint32_t z[GPB]; uint4 x[8]; };
 
-template <int G, int MT, int NW>
+template <int G, int NW>
 __global__ __launch_bounds__(NW * 64) void linear_w4_f32_kernel(W4Args a) {
     constexpr int GPB = 128 / G;
-    const int m0 = blockIdx.y * 16 * MT;
+    const int m0 = blockIdx.y * 16;
     const long nt = blockIdx.x;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
-    __shared__ f32x4 lds[NW * MT * 8 * 64];                              // x of the waves, then their partial sums
-    uint4* xl = reinterpret_cast<uint4*>(lds) + wave * MT * 8 * 64;
+    __shared__ f32x4 lds[NW * 8 * 64];                                   // x of the waves, then their partial sums
+    uint4* xl = reinterpret_cast<uint4*>(lds) + wave * 8 * 64;
     const int pc = lane & 3, rw = lane >> 2;                             // this lane loads pieces pc and pc + 4 (of 8 per fragment) of row rw
-    const int rows = min(a.M - m0, 16 * MT);
+    const int rows = min(a.M - m0, 16);
     const __amdgpu_buffer_rsrc_t xb = buf_rsrc((const float*)a.x + (long)m0 * a.x_rs, (uint32_t)(((rows - 1) * a.x_rs + a.K) * 4));
-    uint32_t xo[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) xo[t] = (uint32_t)(min(t * 16 + rw, rows - 1) * a.x_rs + pc * 4) * 4;
+    const uint32_t xo = (uint32_t)(min(rw, rows - 1) * a.x_rs + pc * 4) * 4;
     const __amdgpu_buffer_rsrc_t wb = buf_rsrc(a.wq + nt * a.KB * 64, a.KB * 1024);
     const __amdgpu_buffer_rsrc_t sb = buf_rsrc((const float*)a.scales + nt * a.KB * GPB * 16, a.KB * GPB * 64);
     const __amdgpu_buffer_rsrc_t zb = buf_rsrc(a.zeros + nt * a.KB * GPB * 16, a.zeros ? a.KB * GPB * 16 : 0);
     const bool has_z = a.zeros != nullptr;
-    typedef W4Stage32<GPB, MT> Stage;
+    typedef W4Stage32<GPB> Stage;
     auto load = [&](Stage& st, int kb) {
         st.w = buf_load16(wb, kb * 1024 + lane * 16);
 #pragma unroll
@@ -280,34 +278,26 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_f32_kernel(W4Args a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int k = kb * 128 + (j >> 1) * 32;
-#pragma unroll
-            for (int t = 0; t < MT; ++t) st.x[t][j] = buf_load16(xb, k < a.K ? xo[t] + kb * 512 + j * 64 : BUF_OFF);
+            st.x[j] = buf_load16(xb, k < a.K ? xo + kb * 512 + j * 64 : BUF_OFF);
         }
     };
-    f32x4 acc[2][MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) acc[0][t] = acc[1][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     auto use = [&](const Stage& st) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int t = 0; t < MT; ++t) xl[((j >> 1) * MT + t) * 128 + w4_place(rw, (j & 1) * 4 + pc)] = st.x[t][j];
+        for (int j = 0; j < 8; ++j) xl[(j >> 1) * 128 + w4_place(rw, (j & 1) * 4 + pc)] = st.x[j];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int g = j * 32 / G;
             const float z = has_z ? (float)((st.z[g] >> ((fr & 3) * 8)) & 255u) : 8.0f;
-            f32x4 x[MT][2];
+            f32x4 x[2];
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) x[t][e] = __builtin_bit_cast(f32x4, xl[(j * MT + t) * 128 + w4_place(fr, 2 * fq + e)]);
+            for (int e = 0; e < 2; ++e) x[e] = __builtin_bit_cast(f32x4, xl[j * 128 + w4_place(fr, 2 * fq + e)]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float w = (w4_value(w4_word(st.w, j), i) - z) * st.s[g];
-#pragma unroll
-                for (int t = 0; t < MT; ++t) acc[i & 1][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, x[t][i >> 2][i & 3], acc[i & 1][t], 0, 0, 0);
+                acc[i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, x[i >> 2][i & 3], acc[i & 1], 0, 0, 0);
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -333,22 +323,20 @@ __global__ __launch_bounds__(NW * 64) void linear_w4_f32_kernel(W4Args a) {
             if (kb + NW < a.KB) use(B);
         }
     }
-    typedef f32x4 part_t[MT][64];
+    typedef f32x4 part_t[64];
     part_t* part = reinterpret_cast<part_t*>(lds);
     __syncthreads();
-#pragma unroll
-    for (int t = 0; t < MT; ++t) part[wave][t][lane] = f32x4{acc[0][t][0] + acc[1][t][0], acc[0][t][1] + acc[1][t][1], acc[0][t][2] + acc[1][t][2], acc[0][t][3] + acc[1][t][3]};
+    part[wave][lane] = f32x4{acc[0][0] + acc[1][0], acc[0][1] + acc[1][1], acc[0][2] + acc[1][2], acc[0][3] + acc[1][3]};
     __syncthreads();
-    for (int i = threadIdx.x; i < MT * 64; i += NW * 64) {
-        const int t = i >> 6, l = i & 63;
-        f32x4 s = part[0][t][l];
+    if (threadIdx.x < 64) {
+        f32x4 s = part[0][lane];
 #pragma unroll
         for (int w = 1; w < NW; ++w) {
-            const f32x4 v = part[w][t][l];
+            const f32x4 v = part[w][lane];
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[r] += v[r];
         }
-        w4_store<float>(a, m0 + t * 16 + (l & 15), nt * 16 + (l >> 4) * 4, s);
+        w4_store<float>(a, m0 + fr, nt * 16 + fq * 4, s);
     }
 }
 
@@ -460,7 +448,7 @@ static void w4_launch(const W4Args& a, int dtype, hipStream_t s) {
     // took 5.6 / 9.8, 9.1 / 5.8 and 23.8 / 27, four more than the matrix form everywhere
     if (a.M == 1) return w4_launch_row<G>(a, s);
     // (two row tiles per workgroup take as long as two workgroups: 55.3 against 2 x 27.2 us at 8192 -> 8192; the MFMAs bound it)
-    linear_w4_f32_kernel<G, 1, 8><<<dim3(ceil_div(a.N, 16), ceil_div(a.M, 16)), 512, 0, s>>>(a);
+    linear_w4_f32_kernel<G, 8><<<dim3(ceil_div(a.N, 16), ceil_div(a.M, 16)), 512, 0, s>>>(a);
 }
 
 extern "C" int valle_linear_w4(const void* x, int64_t x_row_stride, const void* wq, const void* scales, const uint8_t* zeros, const void* bias,

@@ -446,7 +446,7 @@ __global__ __launch_bounds__(128) void rope_kv_paged_kernel(RopePagedArgs a) {
     constexpr int V = 16 / sizeof(T), CH = 64 / V, HS = 128 / CH;       // elements and pieces per head, heads at a time
     const long r = blockIdx.x;
     const int c = threadIdx.x % CH, h0 = threadIdx.x / CH;
-    const int slot = a.slots ? a.slots[r] : -1;
+    const int slot = a.slots[r];
     const int p = min(max(a.pos[r], 0), a.rope_rows - 1);
     float4 cs[V / 4];
 #pragma unroll
