@@ -6,11 +6,12 @@
 // LDS; V is loaded as 4 keys x 4 dims per lane and its 16-bit 4 x 4 blocks are turned in registers (8 v_perm per 16 keys).  The four or eight
 // waves of a workgroup split the keys, so do up to 64 workgroups (grid x) where requests and heads alone do not fill the chip; a second launch
 // joins their partial sums.  Inside the loop waves never wait for one another.
-// Bound: the K / V bytes (2 x T x Hkv x 64 x es) with few queries: 16 requests x 311 .. 761 keys x 16 heads, one token (35 MB) 6.7 us
-// = 5.3 TB/s; 32 x 1,800 .. 2,561 keys, 9 .. 26 nodes (290 MB) 45 us = 6.4 TB/s.  With 64 nodes x 4 grouped heads the bytes no longer
-// count (1 x 130,001 keys: 34 GFLOP in 60 us): without its exponentials that call takes 6 us less, without the P.V products 10, without
-// the loads 12, without K's way through LDS 2 -- two waves per SIMD (244 registers) cover each other's latencies in part.  Tried there and
-// not faster: products placed between the exponentials by scheduling groups, one block's P.V delayed under the next one's exponentials,
+// Bound: the K / V bytes (2 x T x Hkv x 64 x es) with few queries, us on inputs that change from call to call (replayed on the same ones, part of
+// which stays cached): 16 requests x 311 .. 761 keys x 16 heads, one token (35 MB) 9.2 (7.5); 32 x 1,800 .. 2,561 keys, 9 .. 26 nodes
+// (290 MB) 55 (46) = 5.3 TB/s.  With 64 nodes x 4 grouped heads the bytes no longer count (1 x 130,001 keys: 34 GFLOP in 60 us): two waves per
+// SIMD (244 registers) cover each other's latencies in part.  There the vector unit issues in 0.58 of a busy CU's cycles and the matrix unit works in 0.28,
+// waves wait in 0.31 of theirs.  When that call took 69.6 us it took 63.7 without its exponentials, 59.2 without the P.V products, 57.6 without
+// the loads, 68.0 without K's way through LDS.  Tried there and not faster: products placed between the exponentials by scheduling groups, one block's P.V delayed under the next one's exponentials,
 // two loops (with and without masks: spills), query groups of a workgroup sharing tiles, pages of many tiles in one load, tiles requested into
 // L2 two ahead.
 #include "common.h"
@@ -119,9 +120,11 @@ __device__ __forceinline__ void tree_vt(const TreeTile<bf16>& t, bf16x8 (&vt)[4]
     }
 }
 __device__ __forceinline__ void tree_pv(const bf16x8 (&vt)[4], const f32x4 (&p)[2], f32x4 (&o)[4]) {
+    // P is rounded to bf16, the type of V and of the matrix instruction (the denominator keeps fp32): half a step, 2^-8, of each weight.  The result is
+    // 0.0022 .. 0.0024 off the 64-bit one in the 2-norm (its own rounding alone: 0.0017); P in two parts would double the products.
     bf16x8 pf;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) pf[e] = (bf16)p[e >> 2][e & 3];           // P rounded to bf16 for the MFMA (the denominator keeps fp32)
+    for (int e = 0; e < 8; ++e) pf[e] = (bf16)p[e >> 2][e & 3];
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt[dt], pf, o[dt], 0, 0, 0);
 }
@@ -231,8 +234,8 @@ __global__ __launch_bounds__(NW * 64, tree_waves<T>(QB)) void attn_tree_kernel(T
         const int key = (t0 + wave + NW * i) * KT + (lane % NP) * PK;
         return (int)buf_load4(tb, i < mine && key < T_all ? (uint32_t)(key >> a.shift) * 4 : BUF_OFF);
     };
-    // (The scalar work of a tile counts: a descriptor per page and tensor; with one per 16 keys whatever the page 70.5 instead of 67.6 us for
-    // 1 x 130,001 keys, 64 nodes, and 28.4 / 26.2 for 32,768.)
+    // (The scalar work of a tile counts: a descriptor per page and tensor; with one per 16 keys whatever the page 4 % more for 1 x 130,001 keys,
+    // 64 nodes, and 8 % for 32,768, side by side.)
     auto load = [&](Tile& t, int i, int pages) {
         t.live = 0;
         uint32_t ko = lane * 16, vo = (fq * 256 + fr * 4) * (int)sizeof(T);
@@ -502,12 +505,13 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeArgs a) {
     ((T*)a.out)[row * a.o_rs + head * 64 + lane] = from_f32<T>(L == 0.f ? 0.f : acc / L);
 }
 
-// How the work is cut: qb blocks of 16 queries per wave (fp32 tiles leave registers for two), nw waves per workgroup over the keys, `blocks`
+// How the work is cut: qb blocks of 16 queries per wave (up to two in fp32, where 8 registers of the second go through scratch at three waves per
+// SIMD: the sweep below has it so), nw waves per workgroup over the keys, `blocks`
 // workgroups over the queries of a (request, kv head), `split` over its keys.  More blocks per wave save key traffic and the turning of K
 // and V, but hold more registers (four, three, two waves per SIMD at one, two, four blocks) and start and end longer; eight waves finish a
 // request sooner, workgroups of four overlap one's start and end with another's tiles; splitting fills the chip but needs the join.
 // The choice is the least of an estimate in us, fitted to 624 measurements of 33 shapes (it takes 1.3 % more than the best of them, in the
-// mean).  Some of them in bf16, us with qb x nw (requests x context, nodes, heads / kv heads):
+// mean).  Some of them in bf16, us a call in graph replays on the same inputs at the time of that sweep, with qb x nw (requests x context, nodes, heads / kv heads):
 //                                  1 x 4   1 x 8   2 x 4   2 x 8   4 x 4   4 x 8
 //   1 x 130,001, 64, 16/4           114     111      75      74      66      64
 //   32 x 2,200, 64, 16/16            95      93      58      74      52      59

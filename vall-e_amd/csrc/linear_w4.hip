@@ -3,9 +3,11 @@
 // 8-bit float (e4m3), exactly q * 2^-9 -- the subnormals and the first binade are one linear ramp -- so one conversion with a
 // scale of 512 makes two exact bf16 whole numbers.  The MFMA adds up x . q of one group in fp32, another one with an all-ones
 // fragment the sum of the group's x, and the accumulator takes scale * (x.q - zero * sum x) in fp32: no weight is ever rounded.
-// Bound: N K / 2 bytes of weights (plus scales and zeros) while the rows are few: 8192 -> 8192, group 128 (36 MB), 1 .. 16 rows 9.4 us
-// = 3.8 TB/s (8.2 without x's loads); a row tile of 16 more costs 4 us (32 rows 13.4, 40 rows 16.4): x passes through every CU whole,
-// 6 of the 16 us, and the row sums' products another 2.  Small layers are a launch and two round trips: 1024 -> 1024 2.9, 1024 -> 8192 3.5.
+// Bound: N K / 2 bytes of weights (plus scales and zeros) while the rows are few: 8192 -> 8192, group 128 (36 MB), 1 / 16 rows 9.5 / 9.9 us
+// = 3.7 TB/s; every row tile of 16 more costs 4 us (32 rows 13.5, 40 rows 16.5, 64 rows 21.4): x passes through every CU whole and the row sums
+// are computed by every workgroup (40 rows took 16.9 when they took 11.0 without x and 14.9 without the sums).  There the vector unit issues in
+// 0.41 of a busy CU's cycles, the matrix unit works in 0.26, waves wait in 0.32 of theirs.  Small layers are a launch and two round trips:
+// 1024 -> 1024 3.1, 1024 -> 8192 3.5.  (us here and at the choices below: graph replays on the same inputs, both sides in one run.)
 //
 // Layout (the packer writes it once): k blocks of 128, columns in tiles of 16:
 //   wq   [N/16][K/128][64 lanes][16 bytes]: lane l = fq * 16 + fr holds column nt * 16 + fr; its word j (0 .. 3) the weights
@@ -440,6 +442,8 @@ static void w4_launch(const W4Args& a, int dtype, hipStream_t s) {
     if (dtype == VALLE_BF16) {
         // Two column tiles per wave share the row fragments where that leaves a workgroup per CU; us with one / two: 8192 -> 8192, 1 row
         // 10.8 / 9.5, 32 rows 19.9 / 13.4, 40 rows 24.2 / 16.1; 1024 -> 4096, 64 rows 5.7 / 4.3, but 16 rows (128 workgroups of two) 3.1 / 3.5.
+        // (Between 4,096 and 8,192 columns one tile per wave is more than a workgroup per CU, two rounds where the rows fill its LDS: 8192 -> 6144
+        // takes 18.1 us for 32 rows and 23.2 for 40, 8192 -> 8192 13.2 and 16.5.  Two tiles were not measured there.)
         if ((long)ceil_div(a.N, 32) * ceil_div(a.M, 48) >= 256) w4_launch_bf16<G, 2>(a, s);
         else w4_launch_bf16<G, 1>(a, s);
         return;

@@ -121,9 +121,10 @@ __device__ __forceinline__ int plan_lane_scan(int v) {
 // a few dozen cycles; beyond, its first wave, between two barriers), and what the rows need is taken from the state as it was (a page that changes hands in this very call is looked up where it
 // came from), so nobody waits for anybody.  Only the counters may be read and written in one place (n_blocks_out may be n_blocks_in):
 // the last workgroup to have read them, by the ticket, writes them.  The latency is two dependent memory round trips and the ticket's.
-// One workgroup up to 1,024 rows or 16 trees, then one per as many more; us, in the general form / in one workgroup / now: 16 trees of 26
-// nodes 7.3 / 3.5 / 3.6, 64 trees of 26 - / 7.2 / 3.8, 64 prompts of 700 rows - / 6.3 (their rows in a second launch) / 3.9; with E = 8
+// One workgroup up to 1,024 rows or 16 trees, then one per as many more; us when it was built, in the general form / in one workgroup / so: 16
+// trees of 26 nodes 7.3 / 3.5 / 3.6, 64 trees of 26 - / 7.2 / 3.8, 64 prompts of 700 rows - / 6.3 (their rows in a second launch) / 3.9; with E = 8
 // 128 trees of 26 8.3 / - / 5.8, 512 of 8 9.0 / - / 6.3, 512 requests with a row each 6.0 / - / 5.1 (every wave for itself there too: 9.7, 17, 22).
+// 16 trees of 26 and 64 prompts of 305 .. 761 rows, 50 plans in a graph: 4.3 and 3.7.
 template <int E>
 __global__ __launch_bounds__(1024) void page_plan_wave_kernel(PlanArgs a) {
     __shared__ int s_f[64 * E], s_from[64 * E], s_end[64 * E], s_lo[64 * E], s_held[64 * E], s_q[64 * E], s_sum[2];
@@ -412,8 +413,8 @@ extern "C" int valle_page_plan_masked(const int32_t* len_old, const int32_t* len
 // ------------------------------------------------------------------------------------ RoPE + write into pages
 // Elements (2i, 2i + 1) of a q or k head rotate by rope[position][i] = (cos, sin), products and sums in fp32, one rounding at
 // the end (valle_rope_kv rounds cos and sin to bf16 first, as the reference's cast tables are; here the table stays fp32: the
-// result is the formula's within one rounding).  Memory-bound: 2 x 64 x es bytes per head and row.  16 rows of 16 heads 2.2 us (a launch and
-// two round trips: position -> table row; slot), 12,176 rows bf16 (150 MB) 23.5 us = 6.4 TB/s, 28.8 us with caches of other data = 5.2.
+// result is the formula's within one rounding).  Memory-bound: 2 x 64 x es bytes per head and row.  16 rows of 16 heads 2.4 us (a launch and
+// two round trips: position -> table row; slot), 12,176 rows bf16 (150 MB) 23.9 us = 6.3 TB/s, 29.1 us with caches of other data = 5.2.
 struct RopePagedArgs {
     const void *q, *k, *v; void* qo;
     const int32_t* pos; const float* rope; const int32_t* slots;
@@ -508,9 +509,8 @@ extern "C" int valle_rope_kv_paged(const void* q, int64_t q_row_stride, const vo
 // cache[layer][ctx + j] = cache[layer][ctx + path[j]], j < n_accept.  Source and destination ranges overlap: a workgroup reads
 // every row it moves of one (request, head, layer) into registers, meets at a barrier, and writes.  With the plan's status and page counts a
 // request that was not served moves nothing, and no table entry at or behind its page count is followed: such entries are left over
-// and name pages of others.  Three dependent round trips (path,
-// table, row) bound it while the rows are few: one request, 12 layers, 3 rows 2.4 us; 16 requests, 5 rows 4.1; 48 requests, 26 rows (123 MB) 19 us
-// = 6.5 TB/s.
+// and name pages of others.  Three dependent round trips (path, table, row) bound it while the rows are few: one request, 12 layers, 3 rows 2.8 us
+// (2.9 with status and counts); 16 requests, up to 5 rows 4.0 (4.2); 48 requests, 26 rows (123 MB) 22.0 (22.3) = 5.6 TB/s.
 struct CommitArgs {
     void *kc, *vc;
     const int32_t *table, *ctx, *n_blocks, *status, *path, *n_accept;      // n_blocks, status: may be NULL (all entries hold, all were served)

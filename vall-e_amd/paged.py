@@ -101,8 +101,9 @@ def attn_tree(q, k_cache, v_cache, block_table, ctx_len, cu_rows, tree_mask=None
     ``ctx_len[b]`` cached rows and, of the new rows (cached behind them), those whose bit is set in ``tree_mask[row]`` (None: a
     chain, row i sees rows 0 .. i; one row: a plain decode step).  A row that sees nothing is zero.  Requests with a negative
     ``ctx_len`` and rows behind ``cu_rows[-1]`` are left as they were (``out=`` to say what that is; it may be q).  ``max_nodes``: the largest
-    number of rows of a request (default: as many as can be; rows behind it are left), ``max_ctx``: the longest context, a hint
-    for how to split the work."""
+    number of rows of a request (rows behind it are left); the default, min(64, all rows), is right for any batch but cuts the work for trees of that
+    size: a plain decode step passes 1.  ``max_ctx``: the longest context, a hint for how to split the work (default: the table's width).  A prompt of
+    more than 64 rows takes several calls, 64 rows a step; rows beyond are not computed."""
     return _S.attn_tree(q, k_cache, v_cache, block_table, ctx_len, cu_rows, tree_mask, max_nodes, max_ctx,
                         HEAD_DIM ** -0.5 if softmax_scale is None else softmax_scale, out)
 

@@ -113,7 +113,7 @@ class HipLinear4(torch.nn.Module):
     right; from some hundred on a product on unpacked weights is the better choice): ``klass`` for the reference's
     ``replace_linear`` -- constructed as ``klass(in_features, out_features, bias=...)``, a state dict that holds ``weight`` is
     quantised while it loads (vall_e/utils/utils.py:400-428).  ``from_linear`` quantises a module, ``from_quantized`` takes
-    ``quantize_w4``'s layout.  ``forward(x, resid=None, geglu=False)``: + bias, + resid, or gelu(even columns) * odd columns.
+    ``quantize_w4``'s layout; either lays the weights out once, a dozen tensor operations at load.  ``forward(x, resid=None, geglu=False)``: + bias, + resid, or gelu(even columns) * odd columns.
     Weights are not rounded again: whole-number products in fp32 sums, then the scales.  Inference only, as ``HipLinear``."""
 
     GROUPS = (32, 64, 128)
